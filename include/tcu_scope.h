@@ -36,7 +36,8 @@ typedef enum {
   TCU_ERR_CUDA        = 3, /* a CUDA runtime call failed (see cudaGetLastError)         */
   TCU_ERR_TIMEOUT     = 4, /* a bounded device-side wait ran out (tcu_device_error)     */
   TCU_ERR_WORKSPACE   = 5, /* workspace missing or smaller than tcu_workspace_bytes()   */
-  TCU_ERR_TOO_LARGE   = 6  /* more elements than TCU_STATIC_SCAN_MAX_ELEMENTS           */
+  TCU_ERR_TOO_LARGE   = 6, /* more elements than TCU_STATIC_SCAN_MAX_ELEMENTS           */
+  TCU_ERR_INDEX       = 7  /* an index in device memory was wrong (tcu_device_error)    */
 } tcu_status;
 
 typedef enum {
@@ -296,10 +297,116 @@ int tcu_mgpu_full_reduce_f16(tcu_mgpu_ctx* ctx, const void* d_in, float* d_out, 
 int tcu_mgpu_full_scan_f16(tcu_mgpu_ctx* ctx, const void* d_in, void* d_out, int out_type,
                            size_t num_elements, void* stream);
 
+/*
+ * Language-model operators: the scan and the segmented reductions above, with
+ * weights.  A gated linear recurrence is a segmented scan whose running sum
+ * decays; a norm is a segmented sum of squares and its use; the log
+ * probability of a token is a segmented sum of exponentials and its use.
+ * They have no counterpart in the reference.
+ *
+ * Conventions they share, next to those at the top of this file:
+ *   - arguments come in a struct of 8-byte fields; a field left 0 means "not
+ *     given" where it says so;
+ *   - element types are tcu_type codes; everything is computed in 32 bits and
+ *     rounded to the type of the output once;
+ *   - inputs have a stride in elements between rows (any, 0 and negative
+ *     included), the elements of a row lie side by side; outputs are
+ *     contiguous;
+ *   - pointers are aligned to their element's size; 16-byte aligned rows are
+ *     faster;
+ *   - results do not depend on timing: the same call gives the same bits;
+ *   - an index in device memory that is out of range raises bit 3 of
+ *     tcu_device_error, and what it names is left out.
+ */
+typedef enum { TCU_TYPE_F16 = 0, TCU_TYPE_F32 = 1, TCU_TYPE_BF16 = 2 } tcu_type;
+
+/*
+ * Gated linear recurrence along time, for every channel by itself:
+ *     h_t = f_t * h_{t-1} + u_t,    h_{-1} = h0 (0 if not given)
+ *   TCU_GATE_DECAY:    f = a,            u = x
+ *   TCU_GATE_LOG:      f = exp(a),       u = x
+ *   TCU_GATE_SIGMOID:  f = 1/(1+exp(-a)) u = (1 - f) * x
+ * Gates are meant to have |f| <= 1: the product of up to 1024 of them in a
+ * row must stay within float32.
+ *
+ * x, a: `batch` sequences of `tokens` rows of `dim` elements; h: contiguous.
+ * With `offsets` (batch + 1 values, not decreasing, 32- or 64-bit) the
+ * sequences lie one behind the other instead, sequence b being the rows
+ * offsets[b] ... offsets[b+1]-1 of `tokens` rows in all (batch strides
+ * are not used); rows before the first and behind the last sequence are left as
+ * they were, or become 0 where clear_rest is not 0, and a sequence whose offsets are out of range or decrease counts as
+ * empty.  a_type: the type of x, or TCU_TYPE_F32.
+ * h0, last: batch x dim floats; last (may be h0) receives the state behind
+ * each sequence's last row, h0's if the sequence is empty.
+ * states: NULL, or tcu_linear_scan_states_rows() x dim floats that
+ * tcu_linear_scan_backward() wants (the state before every 64th row).
+ */
+typedef enum { TCU_GATE_DECAY = 0, TCU_GATE_LOG = 1, TCU_GATE_SIGMOID = 2 } tcu_gate;
+
+typedef struct {
+  const void* a;
+  const void* x;
+  void* h;
+  const float* h0;     /* may be NULL */
+  float* last;         /* may be NULL */
+  float* states;       /* may be NULL */
+  const void* offsets; /* may be NULL */
+  int64_t batch, tokens, dim;
+  int64_t a_batch_stride, a_row_stride, x_batch_stride, x_row_stride;
+  int64_t gate, a_type, type, offsets_are_64bit, clear_rest;
+} tcu_linear_scan_args;
+int tcu_linear_scan(const tcu_linear_scan_args* args, void* stream);
+
+size_t tcu_linear_scan_states_rows(size_t batch, size_t tokens, int packed);
+
+/*
+ * Its gradient: from dh (of h; may be NULL: zeros), dlast (of last, batch x dim floats; may be
+ * NULL) and the states of the forward call, da and dx (contiguous, in the
+ * types of a and x) and dh0 (batch x dim floats; may be NULL).  a, x, gate and
+ * offsets as in the forward call.
+ */
+typedef struct {
+  const void* dh;
+  const void* a;
+  const void* x;
+  const float* states;
+  const float* dlast; /* may be NULL */
+  void* da;
+  void* dx;
+  float* dh0;          /* may be NULL */
+  const void* offsets; /* may be NULL */
+  int64_t batch, tokens, dim;
+  int64_t dh_batch_stride, dh_row_stride, a_batch_stride, a_row_stride, x_batch_stride, x_row_stride;
+  int64_t gate, a_type, type, offsets_are_64bit, clear_rest;
+} tcu_linear_scan_backward_args;
+int tcu_linear_scan_backward(const tcu_linear_scan_backward_args* args, void* stream);
+
+/*
+ * One token for each of `batch` sequences: row b of a and x advances the state
+ * state[slots[b]] (state: `pool` x dim floats, contiguous, updated in place;
+ * slots NULL: state b) and writes it to row b of h.  A negative slot marks a
+ * padded row: its row of h is left as it was (becomes 0 where clear_rest is not
+ * 0), and so it is, with bit 3 of tcu_device_error, for a slot >= pool and for
+ * one that an earlier row names.
+ */
+typedef struct {
+  const void* a;
+  const void* x;
+  void* h;
+  float* state;
+  const void* slots; /* may be NULL */
+  int64_t batch, pool, dim;
+  int64_t a_row_stride, x_row_stride;
+  int64_t gate, a_type, type, slots_are_64bit, clear_rest;
+} tcu_linear_scan_step_args;
+int tcu_linear_scan_step(const tcu_linear_scan_step_args* args, void* stream);
+
 /* Reads (and optionally clears) the device-side error word of the current
  * device: bit 0 = an mbarrier wait ran out, bit 1 = a tile-status poll ran
- * out, bit 2 = a wait for another GPU's total ran out.  Synchronises the
- * device.  Returns TCU_ERR_TIMEOUT if any bit is set. */
+ * out, bit 2 = a wait for another GPU's total ran out, bit 3 = an index in
+ * device memory was wrong.  Synchronises the device.  Returns
+ * TCU_ERR_TIMEOUT if any of the bits 0 to 2 is set, TCU_ERR_INDEX if bit 3
+ * alone is. */
 int tcu_device_error(unsigned int* bits, int clear);
 
 /*

@@ -14,11 +14,15 @@ from .ops import (  # noqa: E402
     HostContext, TcuError, device_error, fill, full_reduce, full_scan, num_sms, segmented_reduce,
     segmented_scan, workspace_bytes,
 )
+from .lm import (  # noqa: E402
+    linear_scan, linear_scan_backward, linear_scan_states, linear_scan_step,
+)
 from .sharded import PeerGroup, sharded_full_reduce, sharded_full_scan, shard_range  # noqa: E402
 
 __all__ = [
     "ALGO", "DIST", "OP_FULL_REDUCE", "OP_FULL_SCAN", "OP_SEGMENTED_REDUCE", "OP_SEGMENTED_SCAN",
     "HostContext", "TcuError", "device_error", "fill", "full_reduce", "full_scan", "num_sms",
     "segmented_reduce", "segmented_scan", "workspace_bytes", "sharded_full_reduce",
-    "sharded_full_scan", "shard_range", "PeerGroup",
+    "sharded_full_scan", "shard_range", "PeerGroup", "linear_scan", "linear_scan_backward",
+    "linear_scan_states", "linear_scan_step",
 ]

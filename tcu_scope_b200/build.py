@@ -37,6 +37,11 @@ def _newer_than(target: str, sources: list[str]) -> bool:
     return all(os.path.getmtime(s) <= t for s in sources)
 
 
+# The translation units of the library.  capi.cu includes every kernel of the reductions and scans
+# (fp16 inputs), capi_bf16.cu the same sources for bf16 inputs.
+UNITS = ["capi.cu", "capi_bf16.cu", "linear_scan.cu"]
+
+
 def _sources() -> list[str]:
     out = [os.path.join(PKG_DIR, "..", "include", "tcu_scope.h")]
     for name in sorted(os.listdir(CSRC)):
@@ -45,13 +50,12 @@ def _sources() -> list[str]:
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compile csrc/capi.cu (which includes every kernel; fp16 inputs) and csrc/capi_bf16.cu (the
-    same sources for bf16 inputs) into libtcu_scope.so."""
+    """Compile the translation units, side by side, into libtcu_scope.so."""
     srcs = _sources()
     if not force and _newer_than(LIB_PATH, srcs):
         return LIB_PATH
-    cmd = [_nvcc(), *NVCC_FLAGS, "--threads", "2", "-shared", "-o", LIB_PATH,
-           os.path.join(CSRC, "capi.cu"), os.path.join(CSRC, "capi_bf16.cu")]
+    cmd = [_nvcc(), *NVCC_FLAGS, "--threads", str(len(UNITS)), "-shared", "-o", LIB_PATH,
+           *[os.path.join(CSRC, unit) for unit in UNITS]]
     if verbose:
         cmd.insert(1, "-Xptxas")
         cmd.insert(2, "-v")

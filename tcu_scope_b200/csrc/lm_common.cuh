@@ -1,0 +1,114 @@
+// What the language-model operators (linear_scan.cu, norm_residual.cu, token_logprobs.cu) share:
+// element types, vectors of elements, the error word, reductions over a warp and a block.
+// All arithmetic is in 32 bits; a result is rounded to its type once, when it is stored.
+#pragma once
+
+#include "../../include/tcu_scope.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tcu_lm {
+
+constexpr int kMaxDevices = 64;
+
+// Bit of tcu_device_error(): an index in device memory (an offset, a slot, a target) was out of
+// range or named twice; what it names was left out.
+constexpr unsigned kErrIndex = 8u;
+
+// One word for each of the three translation units; tcu_device_error() joins them.
+static __device__ unsigned int g_lm_error_word;
+
+__device__ __forceinline__ void raise_index_error() { atomicOr(&g_lm_error_word, kErrIndex); }
+
+// ------------------------------------------------------------------ elements
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+  return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> zero_vec() {
+  Vec<T, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(0.f);
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
+  Vec<T, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(x[i]);
+  *reinterpret_cast<Vec<T, V>*>(p) = r;
+}
+
+// An index array of 32 or 64 bits.
+__device__ __forceinline__ int64_t load_index(const void* p, int64_t i, bool wide) {
+  return wide ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
+}
+
+// ------------------------------------------------------------------ reductions
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// ------------------------------------------------------------------ host side
+inline int current_device() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -1;
+  return dev >= 0 && dev < kMaxDevices ? dev : -1;
+}
+
+inline int sm_count() {
+  static int counts[kMaxDevices];
+  const int dev = current_device();
+  if (dev < 0) return 0;
+  if (counts[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    counts[dev] = n;
+  }
+  return counts[dev];
+}
+
+inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+inline size_t type_bytes(int64_t type) { return type == TCU_TYPE_F32 ? 4 : 2; }
+
+inline bool known_type(int64_t t) { return t == TCU_TYPE_F16 || t == TCU_TYPE_F32 || t == TCU_TYPE_BF16; }
+
+// Reads (and clears) this translation unit's error word.
+inline int read_error_word(unsigned int* bits, int clear) {
+  unsigned int v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return TCU_ERR_CUDA;
+  if (cudaMemcpyFromSymbol(&v, g_lm_error_word, sizeof(v)) != cudaSuccess) return TCU_ERR_CUDA;
+  if (clear && v) {
+    const unsigned int z = 0;
+    if (cudaMemcpyToSymbol(g_lm_error_word, &z, sizeof(z)) != cudaSuccess) return TCU_ERR_CUDA;
+  }
+  *bits = v;
+  return TCU_OK;
+}
+
+}  // namespace tcu_lm

@@ -1,0 +1,228 @@
+"""Operators of language models next to the reductions and scans: the gated linear recurrence (a scan
+whose running sum decays), with its gradient and its form for single tokens.
+
+Like the other operators these take CUDA tensors, call the C ABI on the current stream of the
+tensors' device and return at once.  They are plain functions: autograd does not record them, so a tensor
+that requires a gradient is refused while autograd records (call under ``torch.no_grad()`` or inside a
+``torch.autograd.Function``), and each has a function for its gradient beside it.  An input may be a view
+with any strides as long as the elements of a row (the last dimension) lie side by side; outputs that
+the caller passes are contiguous and do not overlap other arguments except where it says so.
+"""
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _lib
+from .ops import _check
+
+_TYPE = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+GATE = {"decay": 0, "log": 1, "sigmoid": 2}
+_INDEX = (torch.int32, torch.int64)
+
+
+def _launch(name: str, layout: struct.Struct, fields, device: torch.device) -> None:
+    """Calls an entry point that takes a struct of 8-byte fields, on the tensors' device."""
+    args = layout.pack(*fields)
+    fn = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+    _check(status, name)
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _inputs(device: torch.device, **tensors: torch.Tensor | None) -> None:
+    """What every input has to be: on the device of the first one, and not recorded by autograd."""
+    if device.type != "cuda":
+        raise RuntimeError("input must be a CUDA tensor: there is no CPU path in this library")
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise RuntimeError(f"{name} is on {t.device}, the other tensors on {device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires a gradient, which autograd would not get: call under "
+                               "torch.no_grad() and use the operator's backward function")
+
+
+def _rows(t: torch.Tensor, name: str) -> None:
+    if t.stride(-1) != 1 and t.size(-1) > 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+def _result(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """The caller's output tensor, checked, or a new one."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if t.device != device or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+    return t
+
+
+def _like(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype) -> None:
+    """Checks an optional contiguous input."""
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+
+
+# ------------------------------------------------------------------------------ linear recurrence
+
+_SCAN = struct.Struct("=7Q3q4q5q")
+_SCAN_BACKWARD = struct.Struct("=9Q3q6q5q")
+_STEP = struct.Struct("=5Q3q2q5q")
+
+
+def _scan_shape(a, x, gate, offsets):
+    """(batch, tokens, dim) of a call, after checking what describes it."""
+    if x.dtype not in _TYPE or a.dtype not in (x.dtype, torch.float32):
+        raise TypeError("x must be float16, bfloat16 or float32, a of x's type or float32")
+    if gate not in GATE:
+        raise ValueError(f"gate must be one of {sorted(GATE)}")
+    if a.shape != x.shape:
+        raise ValueError(f"a and x must have one shape, got {tuple(a.shape)} and {tuple(x.shape)}")
+    if offsets is None:
+        if x.dim() != 3:
+            raise ValueError("x must be (batch, tokens, dim), or (tokens, dim) with offsets")
+        batch, tokens, dim = x.shape
+    else:
+        if x.dim() != 2:
+            raise ValueError("x must be (tokens, dim) with offsets")
+        if offsets.dtype not in _INDEX or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
+            raise ValueError("offsets must be a contiguous int32 or int64 tensor of batch + 1 values")
+        (tokens, dim), batch = x.shape, offsets.numel() - 1
+    _rows(a, "a")
+    _rows(x, "x")
+    return batch, tokens, dim
+
+
+def _strides(t: torch.Tensor | None):
+    """(batch stride, row stride)."""
+    if t is None:
+        return 0, 0
+    return (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
+
+
+def linear_scan_states(x: torch.Tensor, offsets: torch.Tensor | None = None) -> torch.Tensor:
+    """An uninitialised tensor for the ``states`` of :func:`linear_scan`: one row of floats for every 64 tokens."""
+    if offsets is None:
+        rows = _lib.load().tcu_linear_scan_states_rows(x.size(0), x.size(1), 0)
+    else:
+        rows = _lib.load().tcu_linear_scan_states_rows(offsets.numel() - 1, x.size(0), 1)
+    return torch.empty((rows, x.size(-1)), dtype=torch.float32, device=x.device)
+
+
+def linear_scan(a: torch.Tensor, x: torch.Tensor, gate: str = "decay", h0: torch.Tensor | None = None,
+                offsets: torch.Tensor | None = None, states: torch.Tensor | None = None,
+                out: torch.Tensor | None = None, last: torch.Tensor | None = None):
+    """The gated linear recurrence ``h[t] = f[t] * h[t-1] + u[t]`` of every channel; returns ``(h, last)``.
+
+    ``gate``: "decay" f = a, u = x; "log" f = exp(a), u = x; "sigmoid" f = sigmoid(a), u = (1 - f) * x.
+    Gates are meant to have ``|f| <= 1`` (products of up to 1024 of them must stay within float32).
+
+    x: (batch, tokens, dim), float16, bfloat16 or float32; a: the same shape, x's type or float32; h: x's shape
+    and type.  h0: float32 (batch, dim), the states before the first tokens (default 0); last: float32
+    (batch, dim), the states behind the last ones (may be h0 itself).
+
+    With ``offsets`` (batch + 1 values, int32 or int64, on the device) x and a are (tokens, dim) and sequence b is their rows
+    ``offsets[b] ... offsets[b+1]-1``.  An empty sequence leaves its state as it is.  Rows outside all
+    sequences are 0 in a new ``h`` and are left as they were in ``out``.  A sequence whose offsets decrease or
+    pass the end counts as empty and raises bit 3 of :func:`device_error`.
+
+    states: from :func:`linear_scan_states`, for :func:`linear_scan_backward`.
+    """
+    device = x.device
+    _inputs(device, x=x, a=a, h0=h0, offsets=offsets, states=states)
+    batch, tokens, dim = _scan_shape(a, x, gate, offsets)
+    _like(h0, "h0", (batch, dim), torch.float32)
+    clear = out is None
+    h = _result(out, "out", x.shape, x.dtype, device)
+    last = _result(last, "last", (batch, dim), torch.float32, device)
+    if states is not None:
+        rows = _lib.load().tcu_linear_scan_states_rows(batch, tokens, 0 if offsets is None else 1)
+        _like(states, "states", (rows, dim), torch.float32)
+    if offsets is not None and batch == 0:
+        return (h.zero_() if clear else h), last
+    _launch("tcu_linear_scan", _SCAN,
+            (_ptr(a), _ptr(x), _ptr(h), _ptr(h0), _ptr(last), _ptr(states), _ptr(offsets), batch, tokens, dim,
+             *_strides(a), *_strides(x), GATE[gate], _TYPE[a.dtype], _TYPE[x.dtype],
+             offsets is not None and offsets.dtype == torch.int64, clear), device)
+    return h, last
+
+
+def linear_scan_backward(dh: torch.Tensor | None, a: torch.Tensor, x: torch.Tensor, states: torch.Tensor,
+                         gate: str = "decay", dlast: torch.Tensor | None = None,
+                         offsets: torch.Tensor | None = None, da: torch.Tensor | None = None,
+                         dx: torch.Tensor | None = None, dh0: torch.Tensor | None = None):
+    """The gradient of :func:`linear_scan`; returns ``(da, dx, dh0)``.
+
+    dh: the gradient of h (x's shape and type; None: zero); dlast: that of ``last`` (None: zero); a, x, gate and
+    offsets: as in the forward call, states: as it left them.  da and dx have the types of a and x, dh0 is float32.
+    Rows outside all sequences have gradient 0 in new tensors and are left as they were in the caller's.
+    """
+    device = x.device
+    _inputs(device, x=x, a=a, dh=dh, states=states, dlast=dlast, offsets=offsets)
+    batch, tokens, dim = _scan_shape(a, x, gate, offsets)
+    if dh is not None:
+        if dh.shape != x.shape or dh.dtype != x.dtype:
+            raise ValueError("dh must have the shape and type of x")
+        _rows(dh, "dh")
+    rows = _lib.load().tcu_linear_scan_states_rows(batch, tokens, 0 if offsets is None else 1)
+    _like(states, "states", (rows, dim), torch.float32)
+    _like(dlast, "dlast", (batch, dim), torch.float32)
+    if offsets is not None and (da is None) != (dx is None):
+        raise ValueError("with offsets, pass both da and dx or neither")
+    clear = da is None
+    da = _result(da, "da", a.shape, a.dtype, device)
+    dx = _result(dx, "dx", x.shape, x.dtype, device)
+    dh0 = _result(dh0, "dh0", (batch, dim), torch.float32, device)
+    if offsets is not None and batch == 0:
+        return (da.zero_(), dx.zero_(), dh0) if clear else (da, dx, dh0)
+    _launch("tcu_linear_scan_backward", _SCAN_BACKWARD,
+            (_ptr(dh), _ptr(a), _ptr(x), _ptr(states), _ptr(dlast), _ptr(da), _ptr(dx), _ptr(dh0), _ptr(offsets),
+             batch, tokens, dim, *_strides(dh), *_strides(a), *_strides(x), GATE[gate], _TYPE[a.dtype],
+             _TYPE[x.dtype], offsets is not None and offsets.dtype == torch.int64, clear), device)
+    return da, dx, dh0
+
+
+def linear_scan_step(a: torch.Tensor, x: torch.Tensor, state: torch.Tensor, gate: str = "decay",
+                     slots: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of :func:`linear_scan` for each of ``batch`` sequences: advances their states in place and returns h.
+
+    a, x: (batch, dim); state: float32 (pool, dim), contiguous; row b advances ``state[slots[b]]`` (slots: int32 or
+    int64; default: ``state[b]``).  A negative slot marks a padded row: its row of h is 0 in a new tensor and
+    left as it was in ``out``.  The same holds, with bit 3 of :func:`device_error`, for a slot past the pool
+    and for a slot that an earlier row names.
+    """
+    device = x.device
+    _inputs(device, x=x, a=a, state=state, slots=slots)
+    if x.dim() != 2 or a.shape != x.shape:
+        raise ValueError("a and x must both be (batch, dim)")
+    if x.dtype not in _TYPE or a.dtype not in (x.dtype, torch.float32):
+        raise TypeError("x must be float16, bfloat16 or float32, a of x's type or float32")
+    if gate not in GATE:
+        raise ValueError(f"gate must be one of {sorted(GATE)}")
+    _rows(a, "a")
+    _rows(x, "x")
+    batch, dim = x.shape
+    if state.dtype != torch.float32 or state.dim() != 2 or state.size(1) != dim or not state.is_contiguous():
+        raise ValueError(f"state must be a contiguous float32 tensor of shape (pool, {dim})")
+    if slots is None:
+        if state.size(0) < batch:
+            raise ValueError("state has fewer rows than x")
+    elif slots.dtype not in _INDEX or tuple(slots.shape) != (batch,) or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous int32 or int64 tensor of batch values")
+    clear = out is None
+    h = _result(out, "out", x.shape, x.dtype, device)
+    if batch and dim:
+        _launch("tcu_linear_scan_step", _STEP,
+                (_ptr(a), _ptr(x), _ptr(h), _ptr(state), _ptr(slots), batch, state.size(0), dim, a.stride(0),
+                 x.stride(0), GATE[gate], _TYPE[a.dtype], _TYPE[x.dtype],
+                 slots is not None and slots.dtype == torch.int64, clear), device)
+    return h

@@ -1,0 +1,146 @@
+"""Calls that the language-model operators refuse: nothing here reaches a GPU."""
+import struct
+
+import pytest
+import torch
+
+INVALID, UNSUPPORTED = 1, 2
+
+
+@pytest.fixture()
+def lib(built_library):
+    import tcu_scope_b200 as tcu
+    return tcu._lib.load()
+
+
+def pack(layout, **fields):
+    """The bytes of an argument struct from its fields' names; what is not named is 0."""
+    return struct.pack(f"={len(layout)}q", *[fields.pop(f, 0) for f in layout]), assert_empty(fields)
+
+
+def assert_empty(fields):
+    assert not fields, fields
+
+
+def fields_of(name):
+    """The fields of a struct of the header, in order."""
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", "tcu_scope.h")).read(), flags=re.S)
+    body = re.search(r"typedef struct \{([^}]*)\} " + name + ";", text).group(1)
+    out = []
+    for line in body.split(";"):
+        words = re.sub(r"\b(const|void|float|double|int64_t)\b|\*", " ", line).replace(",", " ").split()
+        out += words
+    return out
+
+
+SCAN = dict(a=0x1000, x=0x2000, h=0x3000, batch=2, tokens=8, dim=16, type=2, a_type=2)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(type=9), UNSUPPORTED), (dict(a_type=0), UNSUPPORTED), (dict(gate=3), UNSUPPORTED),
+    (dict(a=0), INVALID), (dict(x=0), INVALID), (dict(h=0), INVALID), (dict(x=0x2001), INVALID),
+    (dict(a=0x1002, a_type=1), INVALID), (dict(h0=0x5002), INVALID), (dict(batch=-1), INVALID),
+    (dict(tokens=1 << 41), INVALID), (dict(batch=1 << 30, tokens=1 << 30), INVALID),
+    (dict(offsets=0x7004, offsets_are_64bit=1), INVALID),
+    (dict(batch=0), 0), (dict(dim=0, a=0), 0),
+])
+def test_linear_scan_c_refusals(lib, change, status):
+    args, _ = pack(fields_of("tcu_linear_scan_args"), **{**SCAN, **change})
+    assert lib.tcu_linear_scan(args, None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(states=0), INVALID), (dict(da=0), INVALID), (dict(dx=0x6001), INVALID), (dict(dlast=2), INVALID),
+    (dict(type=7), UNSUPPORTED), (dict(batch=0), 0),
+])
+def test_linear_scan_backward_c_refusals(lib, change, status):
+    base = dict(a=0x1000, x=0x2000, dh=0x3000, states=0x4000, da=0x5000, dx=0x6000, batch=2, tokens=8, dim=16,
+                type=0, a_type=1)
+    args, _ = pack(fields_of("tcu_linear_scan_backward_args"), **{**base, **change})
+    assert lib.tcu_linear_scan_backward(args, None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(pool=1), INVALID), (dict(state=0), INVALID), (dict(state=0x4002), INVALID), (dict(gate=-1), UNSUPPORTED),
+    (dict(batch=0), 0),
+])
+def test_linear_scan_step_c_refusals(lib, change, status):
+    base = dict(a=0x1000, x=0x2000, h=0x3000, state=0x4000, batch=2, pool=2, dim=16, type=1, a_type=1)
+    args, _ = pack(fields_of("tcu_linear_scan_step_args"), **{**base, **change})
+    assert lib.tcu_linear_scan_step(args, None) == status
+
+
+def test_null_arguments(lib):
+    for name in ("tcu_linear_scan", "tcu_linear_scan_backward", "tcu_linear_scan_step"):
+        assert getattr(lib, name)(None, None) == INVALID
+
+
+def test_states_rows(lib):
+    assert lib.tcu_linear_scan_states_rows(3, 64, 0) == 3 and lib.tcu_linear_scan_states_rows(3, 65, 0) == 6
+    assert lib.tcu_linear_scan_states_rows(3, 65, 1) == 4 and lib.tcu_linear_scan_states_rows(3, 0, 0) == 0
+
+
+def test_python_structs_match_the_header(built_library):
+    import tcu_scope_b200.lm as lm
+    for layout, name in ((lm._SCAN, "tcu_linear_scan_args"), (lm._SCAN_BACKWARD, "tcu_linear_scan_backward_args"),
+                         (lm._STEP, "tcu_linear_scan_step_args")):
+        assert layout.size == 8 * len(fields_of(name)), name
+
+
+def test_cpu_tensors_are_refused(built_library):
+    import tcu_scope_b200 as tcu
+    x = torch.zeros(1, 4, 8)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        tcu.linear_scan(x, x)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        tcu.linear_scan_backward(x, x, x, x)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        tcu.linear_scan_step(x[0], x[0], x[0])
+
+
+@pytest.mark.gpu
+def test_linear_scan_python_refusals():
+    import tcu_scope_b200 as tcu
+    x = torch.zeros(2, 4, 8, device="cuda")
+    s = tcu.linear_scan_states(x)
+    with pytest.raises(TypeError):
+        tcu.linear_scan(x.half(), x)
+    with pytest.raises(TypeError):
+        tcu.linear_scan(x.double(), x.double())
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x, x, gate="tanh")
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x[:1], x)
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x[0], x[0])
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x.transpose(1, 2), x.transpose(1, 2))
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x, x, h0=torch.zeros(2, 7, device="cuda"))
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x, x, h0=torch.zeros(2, 8, device="cuda", dtype=torch.float64))
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x, x, states=s[:1])
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x, x, out=torch.zeros(2, 8, 4, device="cuda").transpose(1, 2))
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x, x, offsets=torch.zeros(3, device="cuda", dtype=torch.int32))
+    with pytest.raises(ValueError):
+        tcu.linear_scan(x[0], x[0], offsets=torch.zeros(3, device="cuda"))
+    with pytest.raises(RuntimeError):
+        tcu.linear_scan(x[0], x[0], offsets=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="gradient"):
+        tcu.linear_scan(x, x.clone().requires_grad_())
+    with torch.no_grad():
+        tcu.linear_scan(x, x.clone().requires_grad_())
+    with pytest.raises(ValueError):
+        tcu.linear_scan_backward(x[:, :3], x, x, s)
+    with pytest.raises(ValueError):
+        tcu.linear_scan_backward(x, x, x, s[:1])
+    with pytest.raises(ValueError):
+        tcu.linear_scan_step(x[0], x[0], torch.zeros(3, 8, device="cuda"))
+    with pytest.raises(ValueError):
+        tcu.linear_scan_step(x[0], x[0], torch.zeros(4, 8, device="cuda"), slots=torch.zeros(3, device="cuda", dtype=torch.int32))
