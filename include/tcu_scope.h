@@ -401,6 +401,68 @@ typedef struct {
 } tcu_linear_scan_step_args;
 int tcu_linear_scan_step(const tcu_linear_scan_step_args* args, void* stream);
 
+/*
+ * The norms around a block of a model, fused with its gate and its residual
+ * connection, for `rows` rows of `dim` elements (up to 16384):
+ *     n = z / rms(z) * post_weight                  (z itself without post_weight)
+ *     out = residual + scale * act(gate) * n        (residual 0, act(gate) 1 if not given)
+ *     normed = out / rms(out) * pre_weight          (only with pre_weight)
+ * with rms(y) = sqrt(mean(y^2) + eps), and out not rounded before it is normed.
+ * gate: gate_rows rows, each for rows / gate_rows consecutive rows (1: one
+ * learned vector; rows: a gate for every element); gate_rows divides rows.
+ * type: of z, residual, gate, out and normed; weight_type: that type or
+ * TCU_TYPE_F32.  out may be z's or residual's buffer, normed z's, if that is
+ * contiguous.
+ */
+typedef enum { TCU_ACT_NONE = 0, TCU_ACT_SIGMOID = 1, TCU_ACT_SILU = 2 } tcu_act;
+
+typedef struct {
+  const void* z;
+  const void* residual;    /* may be NULL */
+  const void* post_weight; /* may be NULL */
+  const void* gate;        /* may be NULL */
+  const void* pre_weight;  /* may be NULL */
+  void* out;
+  void* normed;            /* only with pre_weight */
+  int64_t rows, dim, gate_rows;
+  int64_t z_row_stride, residual_row_stride, gate_row_stride;
+  int64_t act, type, weight_type;
+  double scale, eps;
+} tcu_norm_residual_args;
+int tcu_norm_residual(const tcu_norm_residual_args* args, void* stream);
+
+/*
+ * Its gradient: from dout and dnormed (NULL: zeros) dz, and whichever of the
+ * others are not NULL, each in the type of what it is the gradient of.  The
+ * sums over rows are made in a fixed order.  dresidual may be dout's buffer,
+ * dz may be z's, dout's (if that is not dresidual too) or dnormed's, if that is
+ * contiguous.  The workspace is 16-byte aligned, of
+ * tcu_norm_residual_workspace_bytes(), and needs no initialisation.
+ */
+typedef struct {
+  const void* dout;        /* may be NULL */
+  const void* dnormed;     /* may be NULL */
+  const void* z;
+  const void* residual;    /* may be NULL */
+  const void* post_weight; /* may be NULL */
+  const void* gate;        /* may be NULL */
+  const void* pre_weight;  /* may be NULL */
+  void* dz;
+  void* dresidual;         /* may be NULL */
+  void* dpost_weight;      /* may be NULL */
+  void* dgate;             /* may be NULL; gate_rows x dim */
+  void* dpre_weight;       /* may be NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t rows, dim, gate_rows;
+  int64_t dout_row_stride, dnormed_row_stride, z_row_stride, residual_row_stride, gate_row_stride;
+  int64_t act, type, weight_type;
+  double scale, eps;
+} tcu_norm_residual_backward_args;
+int tcu_norm_residual_backward(const tcu_norm_residual_backward_args* args, void* stream);
+
+size_t tcu_norm_residual_workspace_bytes(size_t rows, size_t dim, size_t gate_rows);
+
 /* Reads (and optionally clears) the device-side error word of the current
  * device: bit 0 = an mbarrier wait ran out, bit 1 = a tile-status poll ran
  * out, bit 2 = a wait for another GPU's total ran out, bit 3 = an index in

@@ -15,7 +15,8 @@ from .ops import (  # noqa: E402
     segmented_scan, workspace_bytes,
 )
 from .lm import (  # noqa: E402
-    linear_scan, linear_scan_backward, linear_scan_states, linear_scan_step,
+    NormGradients, linear_scan, linear_scan_backward, linear_scan_states, linear_scan_step, norm_residual,
+    norm_residual_backward,
 )
 from .sharded import PeerGroup, sharded_full_reduce, sharded_full_scan, shard_range  # noqa: E402
 
@@ -24,5 +25,5 @@ __all__ = [
     "HostContext", "TcuError", "device_error", "fill", "full_reduce", "full_scan", "num_sms",
     "segmented_reduce", "segmented_scan", "workspace_bytes", "sharded_full_reduce",
     "sharded_full_scan", "shard_range", "PeerGroup", "linear_scan", "linear_scan_backward",
-    "linear_scan_states", "linear_scan_step",
+    "linear_scan_states", "linear_scan_step", "norm_residual", "norm_residual_backward", "NormGradients",
 ]

@@ -64,6 +64,9 @@ SIGNATURES = {
     "tcu_linear_scan_states_rows": (c_size_t, [c_size_t, c_size_t, c_int]),
     "tcu_linear_scan_backward": (c_int, [c_void_p, c_void_p]),
     "tcu_linear_scan_step": (c_int, [c_void_p, c_void_p]),
+    "tcu_norm_residual": (c_int, [c_void_p, c_void_p]),
+    "tcu_norm_residual_backward": (c_int, [c_void_p, c_void_p]),
+    "tcu_norm_residual_workspace_bytes": (c_size_t, [c_size_t, c_size_t, c_size_t]),
     "tcu_device_error": (c_int, [ctypes.POINTER(ctypes.c_uint), c_int]),
     "tcu_test_set_wait_limits": (c_int, [ctypes.c_uint, ctypes.c_uint, ctypes.c_uint, ctypes.c_uint]),
     "tcu_test_inject": (c_int, [c_int, ctypes.c_ulonglong]),

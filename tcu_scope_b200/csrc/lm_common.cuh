@@ -24,8 +24,9 @@ static __device__ unsigned int g_lm_error_word;
 __device__ __forceinline__ void raise_index_error() { atomicOr(&g_lm_error_word, kErrIndex); }
 
 // ------------------------------------------------------------------ elements
+// (16 bytes are the widest access: longer vectors are several of them)
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Vec {
   T v[V];
 };
 

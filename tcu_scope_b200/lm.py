@@ -1,5 +1,6 @@
 """Operators of language models next to the reductions and scans: the gated linear recurrence (a scan
-whose running sum decays), with its gradient and its form for single tokens.
+whose running sum decays), with its gradient and its form for single tokens, and the norms around a block (sums of
+squares of rows, and their use) fused with its gate and its residual, with their gradient.
 
 Like the other operators these take CUDA tensors, call the C ABI on the current stream of the
 tensors' device and return at once.  They are plain functions: autograd does not record them, so a tensor
@@ -11,6 +12,7 @@ the caller passes are contiguous and do not overlap other arguments except where
 from __future__ import annotations
 
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -19,6 +21,7 @@ from .ops import _check
 
 _TYPE = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 GATE = {"decay": 0, "log": 1, "sigmoid": 2}
+ACT = {"none": 0, "sigmoid": 1, "silu": 2}
 _INDEX = (torch.int32, torch.int64)
 
 
@@ -226,3 +229,144 @@ def linear_scan_step(a: torch.Tensor, x: torch.Tensor, state: torch.Tensor, gate
                  x.stride(0), GATE[gate], _TYPE[a.dtype], _TYPE[x.dtype],
                  slots is not None and slots.dtype == torch.int64, clear), device)
     return h
+
+
+# ------------------------------------------------------------------------------ norms, gate, residual
+
+_NORM = struct.Struct("=7Q3q3q3q2d")
+_NORM_BACKWARD = struct.Struct("=13Qq3q5q3q2d")
+
+
+class NormGradients(NamedTuple):
+    """What :func:`norm_residual_backward` returns; None for what the call did not have."""
+    dz: torch.Tensor
+    dresidual: torch.Tensor | None
+    dpost_weight: torch.Tensor | None
+    dgate: torch.Tensor | None
+    dpre_weight: torch.Tensor | None
+
+
+def _row_stride(t: torch.Tensor | None, name: str) -> int:
+    """The stride between the rows of t (all dimensions but the last, one after the other)."""
+    if t is None:
+        return 0
+    _rows(t, name)
+    if t.dim() == 2:
+        return t.stride(0)
+    if t.is_contiguous() or t.numel() == 0:
+        return t.size(-1)
+    try:
+        return t.view(-1, t.size(-1)).stride(0)
+    except RuntimeError:
+        raise ValueError(f"the rows of {name} must be one stride apart") from None
+
+
+def _norm_arguments(z, residual, post_weight, gate, gate_act, pre_weight):
+    """(rows, dim, gate rows, weight type) of a call, after checking what describes it."""
+    if z.dtype not in _TYPE:
+        raise TypeError("z must be float16, bfloat16 or float32")
+    if z.dim() < 1 or z.size(-1) == 0:
+        raise ValueError("z must have rows of at least one element")
+    if gate_act not in ACT:
+        raise ValueError(f"gate_act must be one of {sorted(ACT)}")
+    dim = z.size(-1)
+    rows = z.numel() // dim
+    if residual is not None and (residual.shape != z.shape or residual.dtype != z.dtype):
+        raise ValueError("residual must have the shape and type of z")
+    weight = post_weight if post_weight is not None else pre_weight
+    w_type = z.dtype if weight is None else weight.dtype
+    if w_type not in (z.dtype, torch.float32):
+        raise TypeError("weights must have z's type or float32")
+    _like(post_weight, "post_weight", (dim,), w_type)
+    _like(pre_weight, "pre_weight", (dim,), w_type)
+    gate_rows = 1
+    if gate is not None:
+        if gate.dtype != z.dtype or gate.dim() < 1 or gate.size(-1) != dim:
+            raise ValueError("gate must have z's type and last dimension")
+        gate_rows = gate.numel() // dim
+        lead, of = tuple(gate.shape[:-1]), tuple(z.shape[:-1])
+        fits = lead == () or (len(of) == 1 and len(lead) == 1 and gate_rows > 0 and rows % gate_rows == 0) or \
+            any(lead == of[:k] + (1,) * (len(of) - k) for k in range(len(of) + 1))
+        if not fits:
+            raise ValueError(f"gate {tuple(gate.shape)} does not give consecutive rows of z {tuple(z.shape)} a gate: "
+                             "it is (dim,), (groups, dim) for a z of groups * n rows, or z's shape with trailing "
+                             "dimensions before the last of size 1")
+    return rows, dim, gate_rows, w_type
+
+
+def norm_residual(z: torch.Tensor, residual: torch.Tensor | None = None, *,
+                  post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                  gate_act: str = "none", scale: float = 1.0, pre_weight: torch.Tensor | None = None,
+                  eps: float = 1e-6, out: torch.Tensor | None = None, normed: torch.Tensor | None = None):
+    """The norm behind a block, its gate, its residual connection and the next block's norm; returns ``(out, normed)``.
+
+    ``out = residual + scale * act(gate) * z / rms(z) * post_weight`` and
+    ``normed = out / rms(out) * pre_weight``, ``rms(y) = sqrt(mean(y * y) + eps)`` of each row (the last dimension, up to
+    16384 elements).  Without post_weight z is not normed, without pre_weight ``normed`` is None; without gate it is 1,
+    without residual 0.  ``normed`` is made from ``out`` before that is rounded.
+
+    z, residual: one shape; float16, bfloat16 or float32; gate: their type, of shape (dim,), of z's
+    shape, of z's shape with 1 in the place of trailing dimensions before the last ((batch, 1, dim) for a z of (batch, tokens, dim)), or,
+    for a z of (rows, dim), (groups, dim): a gate for each of groups * n consecutive rows.  gate_act: "none",
+    "sigmoid" or "silu" of the gate.  Weights: (dim,), z's type or float32.
+    ``out`` may be z or residual themselves, ``normed`` z, if they are contiguous.
+    """
+    device = z.device
+    _inputs(device, z=z, residual=residual, post_weight=post_weight, gate=gate, pre_weight=pre_weight)
+    rows, dim, gate_rows, w_type = _norm_arguments(z, residual, post_weight, gate, gate_act, pre_weight)
+    out = _result(out, "out", z.shape, z.dtype, device)
+    if pre_weight is not None:
+        normed = _result(normed, "normed", z.shape, z.dtype, device)
+    elif normed is not None:
+        raise ValueError("normed needs pre_weight")
+    if rows:
+        _launch("tcu_norm_residual", _NORM,
+                (_ptr(z), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight), _ptr(out), _ptr(normed),
+                 rows, dim, gate_rows, _row_stride(z, "z"), _row_stride(residual, "residual"),
+                 _row_stride(gate, "gate") if gate_rows > 1 else 0, ACT[gate_act], _TYPE[z.dtype], _TYPE[w_type],
+                 scale, eps), device)
+    return out, normed
+
+
+def norm_residual_backward(dout: torch.Tensor | None, dnormed: torch.Tensor | None, z: torch.Tensor,
+                           residual: torch.Tensor | None = None, *, post_weight: torch.Tensor | None = None,
+                           gate: torch.Tensor | None = None, gate_act: str = "none", scale: float = 1.0,
+                           pre_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                           dz: torch.Tensor | None = None, dresidual: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None) -> NormGradients:
+    """The gradient of :func:`norm_residual`, from those of ``out`` and ``normed`` (None: zero).
+
+    The other arguments are those of the forward call.  Each gradient has the shape and type of what it is the
+    gradient of; those of weights and of a gate that rows share are summed over the rows in a fixed order.
+    ``dresidual`` may be dout itself; ``dz`` may be z, dnormed, or, if dresidual is not, dout.
+    """
+    device = z.device
+    _inputs(device, z=z, residual=residual, post_weight=post_weight, gate=gate, pre_weight=pre_weight, dout=dout,
+            dnormed=dnormed, workspace=workspace)
+    rows, dim, gate_rows, w_type = _norm_arguments(z, residual, post_weight, gate, gate_act, pre_weight)
+    for name, t in (("dout", dout), ("dnormed", dnormed)):
+        if t is not None and (t.shape != z.shape or t.dtype != z.dtype):
+            raise ValueError(f"{name} must have the shape and type of z")
+    if dnormed is not None and pre_weight is None:
+        raise ValueError("dnormed needs pre_weight")
+    dz = _result(dz, "dz", z.shape, z.dtype, device)
+    if residual is not None:
+        dresidual = _result(dresidual, "dresidual", z.shape, z.dtype, device)
+    elif dresidual is not None:
+        raise ValueError("dresidual needs residual")
+    dpost = None if post_weight is None else torch.empty_like(post_weight)
+    dpre = None if pre_weight is None else torch.empty_like(pre_weight)
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=device)
+    need = _lib.load().tcu_norm_residual_workspace_bytes(rows, dim, gate_rows)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _launch("tcu_norm_residual_backward", _NORM_BACKWARD,
+            (_ptr(dout), _ptr(dnormed), _ptr(z), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight),
+             _ptr(dz), _ptr(dresidual), _ptr(dpost), _ptr(dgate), _ptr(dpre), _ptr(workspace),
+             workspace.numel() * workspace.element_size(), rows, dim, gate_rows, _row_stride(dout, "dout"),
+             _row_stride(dnormed, "dnormed"), _row_stride(z, "z"), _row_stride(residual, "residual"),
+             _row_stride(gate, "gate") if gate_rows > 1 else 0, ACT[gate_act], _TYPE[z.dtype], _TYPE[w_type], scale,
+             eps), device)
+    return NormGradients(dz, dresidual, dpost, dgate, dpre)

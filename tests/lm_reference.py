@@ -76,3 +76,95 @@ def linear_scan(gate, a, x, h0, dh=None, dlast=None):
         got["dx"] = (g, goff)
     got["dh0"] = (f[0] * g[0], (f[0] * goff[0]).abs() + STEP * gsize[0] * f[0].abs()) if n else (dlast, torch.zeros_like(dlast))
     return got
+
+
+class Run:
+    """A value with a bound on what 32-bit arithmetic may be off: running error analysis.  Every
+    operation carries the bounds of its operands on and adds its own roundings, as many units u of the
+    result's size as are given (1 for a rounded operation, 4 for a function within 2 ulp)."""
+
+    def __init__(self, value, bound=None):
+        self.v = value
+        self.e = torch.zeros_like(value) if bound is None else bound
+
+    def _new(self, value, bound, roundings):
+        return Run(value, bound + roundings * U * (value.abs() + bound))
+
+    def __add__(self, o):
+        return self._new(self.v + o.v, self.e + o.e, 1)
+
+    def __sub__(self, o):
+        return self._new(self.v - o.v, self.e + o.e, 1)
+
+    def __mul__(self, o):
+        if not isinstance(o, Run):
+            o = Run(torch.as_tensor(float(o), dtype=torch.float64).to(self.v.device))
+        return self._new(self.v * o.v, self.v.abs() * o.e + o.v.abs() * self.e + self.e * o.e, 1)
+
+    def call(self, f, slope, roundings=4):
+        """f of the value; slope: a bound on |f'| around it."""
+        return self._new(f(self.v), slope * self.e, roundings)
+
+    def sum(self, dim, keepdim=False, chain=None):
+        """A sum in which every term passes through at most `chain` additions."""
+        n = self.v.shape[dim] if chain is None else chain
+        size = (self.v.abs() + self.e).sum(dim, keepdim=keepdim)
+        return Run(self.v.sum(dim, keepdim=keepdim), self.e.sum(dim, keepdim=keepdim) + n * U * size)
+
+    def index(self, f):
+        return Run(f(self.v), f(self.e))
+
+
+def norm_residual(z, residual, post, gate, act, scale, pre, eps, dout=None, dnormed=None):
+    """Rows of float64 on the CPU, gate expanded to rows or None: {name: Run}; the gradients of post,
+    pre and gate before they are summed over rows are post_rows, pre_rows and gate_rows."""
+    dim = z.shape[1]
+    chain = 16 + 5 + 6  # a thread's elements, its warp, the block's warps
+
+    def scaled(y):  # y / rms(y) and 1 / rms(y)
+        mean = (y * y).sum(1, True, chain) * (1.0 / dim)
+        ms = Run(mean.v + eps, mean.e + U * (mean.v + eps))
+        r = ms.call(lambda m: m.rsqrt(), 0.51 * (ms.v - ms.e).clamp(min=1e-300) ** -1.5)
+        return y * r, r
+
+    got = {}
+    z_ = Run(z)
+    zn, rz = scaled(z_) if post is not None else (z_, None)
+    n = zn * Run(post) if post is not None else zn
+    if gate is not None:
+        sig = torch.sigmoid(gate)
+        value = {"none": gate, "sigmoid": sig, "silu": gate * sig}[act]
+        g = Run(value, 0 * value if act == "none" else 12 * U * value.abs())
+        t = 1 - sig if act != "none" else None
+        slope = {"none": lambda: Run(torch.ones_like(gate)), "sigmoid": lambda: Run(sig * t, 26 * U * sig * t),
+                 "silu": lambda: Run(sig * (1 + gate * t), 30 * U * sig * (1 + (gate * t).abs()))}[act]()
+    else:
+        g = Run(torch.ones_like(z))
+    o = n * g * scale
+    if residual is not None:
+        o = o + Run(residual)
+    got["out"] = o
+    if pre is not None:
+        on, ro = scaled(o)
+        got["normed"] = on * Run(pre)
+    if dout is None:
+        return got
+    d = Run(dout)
+    if pre is not None:
+        v = Run(dnormed) * Run(pre)
+        mean = (v * on).sum(1, True, chain + 2) * (1.0 / dim)
+        got["pre_rows"] = Run(dnormed) * on
+        d = d + ro * (v - on * mean)
+    got["dresidual"] = d
+    ds = d * scale
+    if gate is not None:
+        got["gate_rows"] = ds * n * slope
+    dn = ds * g
+    if post is not None:
+        got["post_rows"] = dn * zn
+        w = dn * Run(post)
+        mean = (w * zn).sum(1, True, chain + 2) * (1.0 / dim)
+        got["dz"] = rz * (w - zn * mean)
+    else:
+        got["dz"] = dn
+    return got

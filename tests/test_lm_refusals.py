@@ -144,3 +144,77 @@ def test_linear_scan_python_refusals():
         tcu.linear_scan_step(x[0], x[0], torch.zeros(3, 8, device="cuda"))
     with pytest.raises(ValueError):
         tcu.linear_scan_step(x[0], x[0], torch.zeros(4, 8, device="cuda"), slots=torch.zeros(3, device="cuda", dtype=torch.int32))
+
+
+NORM = dict(z=0x1000, post_weight=0x2000, out=0x3000, rows=4, dim=64, type=0, weight_type=1)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(type=3), UNSUPPORTED), (dict(weight_type=2), UNSUPPORTED), (dict(act=3), UNSUPPORTED),
+    (dict(dim=16385), UNSUPPORTED), (dict(rows=-1), INVALID), (dict(gate=0x4000, gate_rows=3), INVALID),
+    (dict(gate=0x4000, gate_rows=0), INVALID), (dict(z=0), INVALID), (dict(out=0), INVALID), (dict(z=0x1001), INVALID),
+    (dict(post_weight=0x2002), INVALID), (dict(pre_weight=0x5000), INVALID), (dict(rows=0), 0),
+])
+def test_norm_residual_c_refusals(lib, change, status):
+    args, _ = pack(fields_of("tcu_norm_residual_args"), **{**NORM, **change})
+    assert lib.tcu_norm_residual(args, None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(dz=0), INVALID), (dict(dgate=0x6000), INVALID), (dict(dpre_weight=0x6000), INVALID), (dict(workspace=0), 5),
+    (dict(workspace=0x7008), 5), (dict(workspace_bytes=16), 5), (dict(dresidual=0x8001), INVALID),
+    (dict(rows=0, dpost_weight=0), 0),
+])
+def test_norm_residual_backward_c_refusals(lib, change, status):
+    base = dict(z=0x1000, dout=0x1100, post_weight=0x2000, dz=0x3000, dpost_weight=0x5000, workspace=0x7000,
+                workspace_bytes=1 << 30, rows=4, dim=64, type=0, weight_type=1)
+    args, _ = pack(fields_of("tcu_norm_residual_backward_args"), **{**base, **change})
+    assert lib.tcu_norm_residual_backward(args, None) == status
+
+
+def test_norm_structs_and_workspace(lib):
+    import tcu_scope_b200.lm as lm
+    for layout, name in ((lm._NORM, "tcu_norm_residual_args"), (lm._NORM_BACKWARD, "tcu_norm_residual_backward_args")):
+        assert layout.size == 8 * len(fields_of(name)), name
+    ws = lib.tcu_norm_residual_workspace_bytes
+    assert ws(0, 64, 1) == 0 and ws(10, 0, 1) == 0
+    assert ws(1 << 20, 4096, 1) >= ws(100, 4096, 1) > 0
+    for name in ("tcu_norm_residual", "tcu_norm_residual_backward"):
+        assert getattr(lib, name)(None, None) == INVALID
+
+
+@pytest.mark.gpu
+def test_norm_residual_python_refusals():
+    import tcu_scope_b200 as tcu
+    z = torch.zeros(2, 4, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    for bad in (dict(z=z.double(), post_weight=w), dict(z=z, post_weight=w.half()), dict(z=z, post_weight=w[:7])):
+        with pytest.raises((TypeError, ValueError)):
+            tcu.norm_residual(bad.pop("z"), **bad)
+    with pytest.raises(ValueError):
+        tcu.norm_residual(z, z[:1], post_weight=w)
+    with pytest.raises(ValueError):
+        tcu.norm_residual(z, post_weight=w, gate_act="tanh")
+    for shape in ((1, 4, 8), (4, 8), (3, 8), (2, 4, 1)):  # a gate for each token, broadcast over the batch, is not one of consecutive rows
+        with pytest.raises(ValueError):
+            tcu.norm_residual(z, post_weight=w, gate=torch.zeros(shape, device="cuda"))
+    for shape in ((8,), (1, 1, 8), (2, 1, 8), (2, 4, 8)):
+        tcu.norm_residual(z, post_weight=w, gate=torch.zeros(shape, device="cuda"))
+    with pytest.raises(ValueError):
+        tcu.norm_residual(z, post_weight=w, normed=z)
+    with pytest.raises(ValueError):
+        tcu.norm_residual(z.transpose(1, 2), post_weight=torch.ones(4, device="cuda"))
+    with pytest.raises(ValueError, match="stride"):
+        tcu.norm_residual(torch.zeros(4, 2, 8, device="cuda").transpose(0, 1)[:, :3], post_weight=w)
+    with pytest.raises(tcu.TcuError):
+        tcu.norm_residual(torch.zeros(2, 16385, device="cuda"), post_weight=torch.ones(16385, device="cuda"))
+    with pytest.raises(RuntimeError, match="gradient"):
+        tcu.norm_residual(z, post_weight=w.clone().requires_grad_())
+    with pytest.raises(RuntimeError):
+        tcu.norm_residual(z, post_weight=w.cpu())
+    with pytest.raises(ValueError):
+        tcu.norm_residual_backward(z, z, z, post_weight=w)
+    with pytest.raises(ValueError):
+        tcu.norm_residual_backward(z, None, z, post_weight=w, dresidual=z)
+    with pytest.raises(ValueError):
+        tcu.norm_residual_backward(z[:1], None, z, post_weight=w)
