@@ -463,6 +463,50 @@ int tcu_norm_residual_backward(const tcu_norm_residual_backward_args* args, void
 
 size_t tcu_norm_residual_workspace_bytes(size_t rows, size_t dim, size_t gate_rows);
 
+/*
+ * Log probabilities of given tokens, for `rows` rows of `vocab` logits:
+ *     lse = log sum_j exp(x_j),  logprob = x_target - lse,
+ *     entropy = - sum_j p_j log p_j,  p_j = exp(x_j - lse),
+ * and the `top` (0 ... TCU_MAX_TOP, at most vocab) most probable tokens: their log
+ * probabilities, falling, and indices (ties: the lowest index first; NaN counts as the largest).  Logits of -inf
+ * are tokens left out; a row of nothing else has lse and log probabilities
+ * -inf and entropy 0.  A row with NaN or +inf gives NaN.
+ * targets: 32- or 64-bit; a row whose target is ignore_index has logprob 0,
+ * and so, with bit 3 of tcu_device_error, has one whose target is out of range.
+ */
+#define TCU_MAX_TOP 32
+typedef struct {
+  const void* logits;
+  const void* targets; /* may be NULL if logprob is */
+  float* logprob;      /* rows; may be NULL */
+  float* entropy;      /* rows; may be NULL */
+  float* lse;          /* rows; may be NULL */
+  float* top_logprob;  /* rows x top */
+  int64_t* top_index;  /* rows x top */
+  int64_t rows, vocab, row_stride, top, ignore_index;
+  int64_t type, targets_are_64bit;
+} tcu_token_logprobs_args;
+int tcu_token_logprobs(const tcu_token_logprobs_args* args, void* stream);
+
+/*
+ * Its gradient: from dlogprob and dentropy (rows floats each; NULL: zeros) and
+ * the lse and entropy of the forward call, dlogits (contiguous, the type of the
+ * logits; may be their buffer if that is contiguous).  Rows whose target counts
+ * for nothing have no part of dlogprob; a row of -inf has gradient 0.
+ */
+typedef struct {
+  const void* logits;
+  const void* targets;   /* may be NULL if dlogprob is */
+  const float* lse;
+  const float* entropy;  /* may be NULL if dentropy is */
+  const float* dlogprob; /* may be NULL */
+  const float* dentropy; /* may be NULL */
+  void* dlogits;
+  int64_t rows, vocab, row_stride, ignore_index;
+  int64_t type, targets_are_64bit;
+} tcu_token_logprobs_backward_args;
+int tcu_token_logprobs_backward(const tcu_token_logprobs_backward_args* args, void* stream);
+
 /* Reads (and optionally clears) the device-side error word of the current
  * device: bit 0 = an mbarrier wait ran out, bit 1 = a tile-status poll ran
  * out, bit 2 = a wait for another GPU's total ran out, bit 3 = an index in

@@ -15,8 +15,8 @@ from .ops import (  # noqa: E402
     segmented_scan, workspace_bytes,
 )
 from .lm import (  # noqa: E402
-    NormGradients, linear_scan, linear_scan_backward, linear_scan_states, linear_scan_step, norm_residual,
-    norm_residual_backward,
+    NormGradients, TokenLogprobs, linear_scan, linear_scan_backward, linear_scan_states, linear_scan_step,
+    norm_residual, norm_residual_backward, token_logprobs, token_logprobs_backward,
 )
 from .sharded import PeerGroup, sharded_full_reduce, sharded_full_scan, shard_range  # noqa: E402
 
@@ -26,4 +26,5 @@ __all__ = [
     "segmented_reduce", "segmented_scan", "workspace_bytes", "sharded_full_reduce",
     "sharded_full_scan", "shard_range", "PeerGroup", "linear_scan", "linear_scan_backward",
     "linear_scan_states", "linear_scan_step", "norm_residual", "norm_residual_backward", "NormGradients",
+    "token_logprobs", "token_logprobs_backward", "TokenLogprobs",
 ]

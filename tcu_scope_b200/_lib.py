@@ -67,6 +67,8 @@ SIGNATURES = {
     "tcu_norm_residual": (c_int, [c_void_p, c_void_p]),
     "tcu_norm_residual_backward": (c_int, [c_void_p, c_void_p]),
     "tcu_norm_residual_workspace_bytes": (c_size_t, [c_size_t, c_size_t, c_size_t]),
+    "tcu_token_logprobs": (c_int, [c_void_p, c_void_p]),
+    "tcu_token_logprobs_backward": (c_int, [c_void_p, c_void_p]),
     "tcu_device_error": (c_int, [ctypes.POINTER(ctypes.c_uint), c_int]),
     "tcu_test_set_wait_limits": (c_int, [ctypes.c_uint, ctypes.c_uint, ctypes.c_uint, ctypes.c_uint]),
     "tcu_test_inject": (c_int, [c_int, ctypes.c_ulonglong]),

@@ -806,14 +806,16 @@ int tcu_wait_limits_of_this_build(const unsigned int* four) {
 #if !TCU_BF16
 // And the error words of the language-model operators, in translation units of their own.
 int tcu_error_word_linear_scan(unsigned int* bits, int clear);
+int tcu_error_word_token_logprobs(unsigned int* bits, int clear);
 
 int tcu_device_error(unsigned int* bits, int clear) {
-  unsigned int a = 0, b = 0, c = 0;
+  unsigned int a = 0, b = 0, c = 0, d = 0;
   if (tcu_error_word_f16_build(&a, clear) != TCU_OK) return TCU_ERR_CUDA;
   if (tcu_error_word_bf16_build(&b, clear) != TCU_OK) return TCU_ERR_CUDA;
   if (tcu_error_word_linear_scan(&c, clear) != TCU_OK) return TCU_ERR_CUDA;
-  if (bits) *bits = a | b | c;
-  return (a | b) ? TCU_ERR_TIMEOUT : c ? TCU_ERR_INDEX : TCU_OK;
+  if (tcu_error_word_token_logprobs(&d, clear) != TCU_OK) return TCU_ERR_CUDA;
+  if (bits) *bits = a | b | c | d;
+  return (a | b) ? TCU_ERR_TIMEOUT : (c | d) ? TCU_ERR_INDEX : TCU_OK;
 }
 
 int tcu_test_set_wait_limits(unsigned barrier_attempts, unsigned status_polls, unsigned flag_polls,

@@ -1,6 +1,7 @@
 """Operators of language models next to the reductions and scans: the gated linear recurrence (a scan
 whose running sum decays), with its gradient and its form for single tokens, and the norms around a block (sums of
-squares of rows, and their use) fused with its gate and its residual, with their gradient.
+squares of rows, and their use) fused with its gate and its residual, with their gradient, and the log
+probabilities of given tokens (sums of exponentials of rows) with entropy and best alternatives, with their gradient.
 
 Like the other operators these take CUDA tensors, call the C ABI on the current stream of the
 tensors' device and return at once.  They are plain functions: autograd does not record them, so a tensor
@@ -370,3 +371,87 @@ def norm_residual_backward(dout: torch.Tensor | None, dnormed: torch.Tensor | No
              _row_stride(gate, "gate") if gate_rows > 1 else 0, ACT[gate_act], _TYPE[z.dtype], _TYPE[w_type], scale,
              eps), device)
     return NormGradients(dz, dresidual, dpost, dgate, dpre)
+
+
+# ------------------------------------------------------------------------------ log probabilities
+
+_LOGPROBS = struct.Struct("=7Q5q2q")
+_LOGPROBS_BACKWARD = struct.Struct("=7Q4q2q")
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns: float32, top_index int64."""
+    logprob: torch.Tensor | None
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_logprob: torch.Tensor | None
+    top_index: torch.Tensor | None
+
+
+def _logits_rows(logits, targets):
+    """(rows, vocab, row stride) of a call, after checking what describes it."""
+    if logits.dtype not in _TYPE:
+        raise TypeError("logits must be float16, bfloat16 or float32")
+    if logits.dim() < 1 or logits.size(-1) == 0:
+        raise ValueError("logits must have rows of at least one element")
+    lead = logits.shape[:-1]
+    if targets is not None and (targets.dtype not in _INDEX or targets.shape != lead or not targets.is_contiguous()):
+        raise ValueError(f"targets must be a contiguous int32 or int64 tensor of shape {tuple(lead)}")
+    return lead.numel(), logits.size(-1), _row_stride(logits, "logits")
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Log probabilities of the target tokens under softmax(logits), with entropy and the ``top`` best alternatives.
+
+    logits: (..., vocab), float16, bfloat16 or float32; targets: (...), int32 or int64 (None: no ``logprob``).
+    Returns ``logprob`` (...), ``entropy`` (...), ``lse`` (...), the log of the sum of exponentials, and, with ``top`` (at most 32)
+    above 0, ``top_logprob`` and ``top_index`` (..., top): the most probable tokens, the most probable first, the lowest index first
+    where they are equal; NaN counts as the largest.
+
+    Logits of -inf are tokens left out.  A row of nothing else has ``lse`` and log probabilities -inf and entropy 0; a
+    row with NaN or +inf gives NaN.  A row whose target is ``ignore_index`` has ``logprob`` 0, and so, with bit
+    3 of :func:`device_error`, has one whose target is out of range.
+    """
+    device = logits.device
+    _inputs(device, logits=logits, targets=targets)
+    rows, vocab, stride = _logits_rows(logits, targets)
+    if top > vocab:
+        raise ValueError("top is more than the vocabulary")
+    lead = logits.shape[:-1]
+    sums = torch.empty((3, *lead), dtype=torch.float32, device=device)
+    lse, entropy = sums[0], sums[1]
+    logprob = sums[2] if targets is not None else None
+    top_logprob = torch.empty((*lead, top), dtype=torch.float32, device=device) if top else None
+    top_index = torch.empty((*lead, top), dtype=torch.int64, device=device) if top else None
+    if rows:
+        _launch("tcu_token_logprobs", _LOGPROBS,
+                (_ptr(logits), _ptr(targets), _ptr(logprob), _ptr(entropy), _ptr(lse), _ptr(top_logprob),
+                 _ptr(top_index), rows, vocab, stride, top, ignore_index, _TYPE[logits.dtype],
+                 targets is not None and targets.dtype == torch.int64), device)
+    return TokenLogprobs(logprob, entropy, lse, top_logprob, top_index)
+
+
+def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor | None, lse: torch.Tensor,
+                            entropy: torch.Tensor | None = None, *, dlogprob: torch.Tensor | None = None,
+                            dentropy: torch.Tensor | None = None, ignore_index: int = -100,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of the logits of :func:`token_logprobs`, from those of ``logprob`` and ``entropy`` (None: zero).
+
+    lse and entropy: as the forward call returned them (entropy is wanted with dentropy, targets with dlogprob).
+    ``out`` may be the logits themselves, if they are contiguous.
+    """
+    device = logits.device
+    _inputs(device, logits=logits, targets=targets, lse=lse, entropy=entropy, dlogprob=dlogprob, dentropy=dentropy)
+    rows, vocab, stride = _logits_rows(logits, targets)
+    for name, t in (("lse", lse), ("entropy", entropy), ("dlogprob", dlogprob), ("dentropy", dentropy)):
+        _like(t, name, logits.shape[:-1], torch.float32)
+    if (dlogprob is not None and targets is None) or (dentropy is not None and entropy is None):
+        raise ValueError("dlogprob needs targets, dentropy needs entropy")
+    out = _result(out, "out", logits.shape, logits.dtype, device)
+    if rows:
+        _launch("tcu_token_logprobs_backward", _LOGPROBS_BACKWARD,
+                (_ptr(logits), _ptr(targets), _ptr(lse), _ptr(entropy), _ptr(dlogprob), _ptr(dentropy), _ptr(out),
+                 rows, vocab, stride, ignore_index, _TYPE[logits.dtype],
+                 targets is not None and targets.dtype == torch.int64), device)
+    return out

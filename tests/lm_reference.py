@@ -168,3 +168,48 @@ def norm_residual(z, residual, post, gate, act, scale, pre, eps, dout=None, dnor
     else:
         got["dz"] = dn
     return got
+
+
+def token_logprobs(x, targets, top, dlp=None, dent=None):
+    """Rows of float64 on the CPU: {name: (value, bound)}, top_index without a bound.  The bounds count the
+    roundings of x - r (u |x - r|), its product (u) and 2^d (4 u) into each exponential, the chain of additions,
+    and the logarithm's 2 ulp."""
+    rows, vocab = x.shape
+    most = x.max(1, keepdim=True).values
+    dead = torch.isinf(most)                      # nothing but -inf
+    far = torch.where(dead | torch.isinf(x), torch.zeros_like(x), x - torch.where(dead, 0.0, most))
+    p = torch.where(dead, torch.zeros_like(x), torch.softmax(torch.where(dead, 0.0, x), 1))
+    logp = torch.where(dead | torch.isinf(x), torch.zeros_like(x), torch.log_softmax(torch.where(dead, 0.0, x), 1))
+    chain = vocab / 128 + 60                      # additions and rebasings a term passes through
+    # what d = (x - r) log2(e) is off, in natural units, weighted: the relative error of s
+    rel = (p * (6 * far.abs() + 8) * U).sum(1) + chain * U
+    log_s = torch.where(dead[:, 0], 0.0, (torch.logsumexp(torch.where(dead, 0.0, x), 1) - torch.where(dead[:, 0], 0.0, most[:, 0])))
+    lse = torch.where(dead[:, 0], most[:, 0], torch.logsumexp(torch.where(dead, 0.0, x), 1))
+    off = rel + 8 * U * (log_s + 1)               # of log s
+    got = {"lse": (lse, off + U * torch.where(dead[:, 0], 0.0, lse.abs())),
+           "entropy": (-(p * logp).sum(1), off + (p * far.abs() * (6 * far.abs() + chain + 12) * U).sum(1) + 4 * U * (log_s + 1) + (p * far.abs()).sum(1) * rel)}
+    row = torch.arange(rows)
+    if targets is not None:
+        t = targets.clamp(0, vocab - 1)
+        got["logprob"] = (torch.where(torch.isinf(x[row, t]), -torch.inf, logp[row, t]), off + 4 * U * (far[row, t].abs() + log_s))
+    if top:
+        order = torch.where(torch.isnan(x), torch.inf, x).sort(dim=1, descending=True, stable=True).indices[:, :top]
+        got["top_index"] = order
+        got["top_logprob"] = (torch.where(torch.isinf(x.gather(1, order)), -torch.inf, logp.gather(1, order)),
+                              off[:, None] + 4 * U * (far.gather(1, order).abs() + log_s[:, None]))
+    if dlp is not None:
+        hit = torch.zeros_like(x)
+        hit[row, targets] = 1
+        hit[dead[:, 0]] = 0
+        ent = got["entropy"][0]
+        g = dlp[:, None] * (hit - p) - dent[:, None] * p * (logp + ent[:, None])
+        # log p from lse: its rounding (or 2^-16 at most), x - lse, the product, and the exponential
+        lost = off + torch.where(dead[:, 0], 0.0, torch.minimum(lse.abs(), torch.full_like(lse, 256.0))) * U
+        rel_p = lost[:, None] + (4 * logp.abs() + 8) * U
+        size = dlp.abs()[:, None] + dent.abs()[:, None] * (logp.abs() + ent[:, None])
+        got["dlogits"] = (g, p * (size * (rel_p + 6 * U) + dent.abs()[:, None] * (lost[:, None] + got["entropy"][1][:, None] + 4 * U * logp.abs()))
+                          + 2 * U * (hit * dlp[:, None].abs())
+                          # a probability below float32's smallest normal number, 2^-126, counts as 0, so p is off by
+                          # less than that, and p (dlp + dH (log p + H)) by less than that times the bracket
+                          + 2.0 ** -126 * size)
+    return got

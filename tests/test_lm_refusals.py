@@ -218,3 +218,68 @@ def test_norm_residual_python_refusals():
         tcu.norm_residual_backward(z, None, z, post_weight=w, dresidual=z)
     with pytest.raises(ValueError):
         tcu.norm_residual_backward(z[:1], None, z, post_weight=w)
+
+
+LOGPROBS = dict(logits=0x1000, targets=0x2000, logprob=0x3000, entropy=0x4000, lse=0x5000, rows=3, vocab=100,
+                row_stride=100, type=2, targets_are_64bit=1)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(type=5), UNSUPPORTED), (dict(top=33, vocab=200), UNSUPPORTED), (dict(top=-1), UNSUPPORTED),
+    (dict(top=4), INVALID), (dict(top=4, vocab=3, top_logprob=0x6000, top_index=0x7000), INVALID),
+    (dict(top=4, top_logprob=0x6000, top_index=0x7004), INVALID), (dict(targets=0), INVALID), (dict(targets=0x2004), INVALID),
+    (dict(logits=0), INVALID), (dict(logits=0x1001), INVALID), (dict(vocab=0), INVALID), (dict(rows=-1), INVALID),
+    (dict(vocab=1 << 31), INVALID), (dict(rows=1 << 31), INVALID), (dict(lse=0x5002), INVALID), (dict(rows=0), 0),
+])
+def test_token_logprobs_c_refusals(lib, change, status):
+    args, _ = pack(fields_of("tcu_token_logprobs_args"), **{**LOGPROBS, **change})
+    assert lib.tcu_token_logprobs(args, None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(lse=0), INVALID), (dict(dlogits=0), INVALID), (dict(dlogits=0x6001), INVALID), (dict(targets=0), INVALID),
+    (dict(dentropy=0x8000, entropy=0), INVALID), (dict(type=-1), UNSUPPORTED), (dict(rows=0), 0),
+])
+def test_token_logprobs_backward_c_refusals(lib, change, status):
+    base = dict(logits=0x1000, targets=0x2000, lse=0x3000, entropy=0x4000, dlogprob=0x5000, dlogits=0x6000, rows=3,
+                vocab=100, row_stride=100, type=0)
+    args, _ = pack(fields_of("tcu_token_logprobs_backward_args"), **{**base, **change})
+    assert lib.tcu_token_logprobs_backward(args, None) == status
+
+
+def test_logprob_structs(lib):
+    import tcu_scope_b200.lm as lm
+    for layout, name in ((lm._LOGPROBS, "tcu_token_logprobs_args"), (lm._LOGPROBS_BACKWARD, "tcu_token_logprobs_backward_args")):
+        assert layout.size == 8 * len(fields_of(name)), name
+    for name in ("tcu_token_logprobs", "tcu_token_logprobs_backward"):
+        assert getattr(lib, name)(None, None) == INVALID
+
+
+@pytest.mark.gpu
+def test_token_logprobs_python_refusals():
+    import tcu_scope_b200 as tcu
+    x, t = torch.zeros(3, 50, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError):
+        tcu.token_logprobs(x.double(), t)
+    for bad in (t[:2], t.float(), t[:, None]):
+        with pytest.raises(ValueError):
+            tcu.token_logprobs(x, bad)
+    with pytest.raises(RuntimeError):
+        tcu.token_logprobs(x, t.cpu())
+    with pytest.raises(ValueError):
+        tcu.token_logprobs(x, t, top=51)
+    with pytest.raises(tcu.TcuError):
+        tcu.token_logprobs(x, t, top=33)
+    with pytest.raises(ValueError):
+        tcu.token_logprobs(x.t(), torch.zeros(50, dtype=torch.int64, device="cuda"))
+    with pytest.raises(RuntimeError, match="gradient"):
+        tcu.token_logprobs(x.clone().requires_grad_(), t)
+    got = tcu.token_logprobs(x, t)
+    with pytest.raises(ValueError):
+        tcu.token_logprobs_backward(x, None, got.lse, got.entropy, dlogprob=got.lse)
+    with pytest.raises(ValueError):
+        tcu.token_logprobs_backward(x, t, got.lse, dentropy=got.lse)
+    with pytest.raises(ValueError):
+        tcu.token_logprobs_backward(x, t, got.lse[:2], got.entropy, dlogprob=got.lse)
+    with pytest.raises(ValueError):
+        tcu.token_logprobs_backward(x, t, got.lse, got.entropy, dlogprob=got.lse, out=x.half())
