@@ -464,7 +464,7 @@ int tcu_norm_residual_backward(const tcu_norm_residual_backward_args* args, void
 size_t tcu_norm_residual_workspace_bytes(size_t rows, size_t dim, size_t gate_rows);
 
 /*
- * Log probabilities of given tokens, for `rows` rows of `vocab` logits:
+ * Log probabilities of given tokens, for `rows` rows of `vocab` (up to 2^30) logits:
  *     lse = log sum_j exp(x_j),  logprob = x_target - lse,
  *     entropy = - sum_j p_j log p_j,  p_j = exp(x_j - lse),
  * and the `top` (0 ... TCU_MAX_TOP, at most vocab) most probable tokens: their log
