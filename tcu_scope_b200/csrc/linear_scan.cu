@@ -3,19 +3,21 @@
 // The step h -> f h + u is a linear map, and maps compose: (A2, H2) after (A1, H1) is
 // (A2 A1, A2 H1 + H2).  So time is cut into pieces whose maps are computed independently, and
 // only the maps are passed along:
-//   - a warp holds 8 consecutive rows of 32 * VEC channels in registers and computes their map;
-//   - the 8 warps of a block hold 64 consecutive rows (a chunk) and exchange maps in shared memory;
-//   - the P blocks of a cluster hold P consecutive chunks (a window) of the same channels and
+//   - a warp takes 16 consecutive rows of 64 channels, two channels a lane, and computes their map;
+//   - the warps of a block take consecutive rows (64 with 4 warps) and exchange maps in shared memory;
+//   - the P blocks of a cluster take consecutive rows of the same channels (a window) and
 //     exchange maps in each other's shared memory;
-//   - the cluster goes through its sequence window by window, the state in registers, the next window's
-//     rows already on their way.
-// Every element is read and written once.  All maps are joined in the order of time, so the result does not depend on timing.
+//   - the cluster goes through its sequence window by window, the state in registers.
+// Every element is read from and written to memory once.  All maps are joined in the order of time, so the
+// result does not depend on timing.
 //
 // Backwards, with g_t = f_t dh_t passing from row t to row t-1 (dh_t = dy_t + g_{t+1}) the same
-// holds with time reversed; h_{t-1} is recomputed from the state before each chunk, which the
+// holds with time reversed; h_{t-1} is recomputed from the state before every 64th row, which the
 // forward pass leaves behind (one row of floats for 64 rows of elements).
 //
-// Bound by HBM: 3 arrays forward, 5 backward.
+// Bound by HBM: 3 arrays forward, 5 backward.  Each warp copies its rows into a ring of its own in shared memory
+// (cp.async, 16 bytes a lane), some windows ahead: nothing but its own copies is waited for, and the
+// registers hold the gates of the current window only.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -27,10 +29,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps      = 8;
-constexpr int kRows       = 8;               // rows per warp and window
-constexpr int kChunk      = kWarps * kRows;  // rows per block and window; also the spacing of the states
+constexpr int kRows       = 16;   // rows per warp and window
+constexpr int kWidth      = 64;   // channels per block
+constexpr int kChunk      = 64;   // spacing of the states
+constexpr int kChunkWarps = kChunk / kRows;
+constexpr int kMaxWarps   = 8;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxStages  = 6;    // windows in a warp's ring
+constexpr int kForwardBlocks = 2, kBackwardBlocks = 2;  // of 8 warps to an SM: 128 registers a thread
 
 struct ScanArgs {
   const void *a, *x, *dh;
@@ -40,24 +46,26 @@ struct ScanArgs {
   const void* offsets;
   int64_t batch, tokens, dim;
   int64_t a_batch, a_row, x_batch, x_row, dh_batch, dh_row;
-  int columns;
+  int columns, stages;
+  int a_piece, x_piece, dh_piece;  // bytes that can be copied at a time: 16, 4 or an element
+  bool pairs;                      // outputs can be written two elements at a time
   bool wide;
   bool clear_rest;  // with offsets: rows outside all sequences become 0
 };
 
-// f and u of one element, and 1 - f (SIGMOID only), computed without cancellation.
+// f of one element, and 1 - f (SIGMOID only), computed without cancellation.  exp(a) = 2^(a log2(e)): the product's
+// rounding makes f off by |a| half steps, relative, which is where f is small and counts for little.
 template <int GATE>
-__device__ __forceinline__ void gate_of(float a, float x, float& f, float& u, float& one_minus_f) {
+__device__ __forceinline__ void gate_of(float a, float& f, float& one_minus_f) {
   if constexpr (GATE == TCU_GATE_SIGMOID) {
-    const float e = expf(-fabsf(a));
-    const float r = __fdividef(1.f, 1.f + e);
+    const float e = exp2_fast(-fabsf(a) * kLog2E);
+    const float r = reciprocal(1.f + e);
     const float s = e * r;
     f           = a >= 0.f ? r : s;
     one_minus_f = a >= 0.f ? s : r;
-    u           = one_minus_f * x;
+    if (a != a) f = one_minus_f = a;
   } else {
-    f = GATE == TCU_GATE_LOG ? expf(a) : a;
-    u = x;
+    f = GATE == TCU_GATE_LOG ? exp2_fast(a * kLog2E) : a;
   }
 }
 
@@ -93,317 +101,404 @@ __device__ __forceinline__ Sequence sequence_of(const ScanArgs& p, int64_t b) {
   return s;
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_rows(Vec<T, VEC> (&r)[kRows], const T* base, int64_t row_stride,
-                                          int64_t row, int64_t length, bool in_dim) {
+// ------------------------------------------------------------------ the ring
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Returns when all but the newest `pending` groups of this thread have arrived.
+__device__ __forceinline__ void copy_wait(int pending) {
+  switch (pending) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+  }
+}
+
+// Copies rows row ... row + 15 (those that are below `length`) of the warp's channels, the first `left` of them,
+// to `to`, kWidth elements a row.  `base`: the block's first channel in the sequence's first row.
+template <typename T>
+__device__ __forceinline__ void copy_rows(T* to, const T* base, int64_t row_stride, int64_t row, int64_t length,
+                                          int left, int piece) {
+  const int lane = threadIdx.x & 31;
+  const int rows = length - row < kRows ? int(length - row) : kRows;  // may be negative
+  const T* from  = base + row * row_stride;
+  if (piece == 16) {
+    constexpr int kLanes = kWidth * int(sizeof(T)) / 16, kAtOnce = 32 / kLanes, kElems = 16 / int(sizeof(T));
+    const int r0 = lane / kLanes, c = lane % kLanes * kElems;
+    if (c >= left) return;
+    from += r0 * row_stride + c;
+    to += r0 * kWidth + c;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i)
-    r[i] = in_dim && row + i < length ? load_vec<T, VEC>(base + (row + i) * row_stride) : zero_vec<T, VEC>();
+    for (int i = 0; i < kRows; i += kAtOnce, from += kAtOnce * row_stride, to += kAtOnce * kWidth)
+      if (i + r0 < rows) copy_async16(to, from);
+  } else if (piece == 4) {
+    constexpr int kElems = 4 / int(sizeof(T));
+#pragma unroll 4
+    for (int i = 0; i < kRows; ++i, from += row_stride, to += kWidth)
+#pragma unroll
+      for (int c = lane * kElems; c < kWidth; c += 32 * kElems)
+        if (i < rows && c < left) copy_async4(to + c, from + c);
+  } else {
+    T x[kRows / 2][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int i = 0; i < kRows / 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (half * (kRows / 2) + i < rows && lane + 32 * k < left) x[i][k] = from[i * row_stride + lane + 32 * k];
+#pragma unroll
+      for (int i = 0; i < kRows / 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (half * (kRows / 2) + i < rows && lane + 32 * k < left) to[i * kWidth + lane + 32 * k] = x[i][k];
+      from += kRows / 2 * row_stride;
+      to += kRows / 2 * kWidth;
+    }
+  }
+}
+
+// A lane's two channels of a row in shared memory.
+template <typename T>
+__device__ __forceinline__ float2 pair_at(const T* row) {
+  const Vec<T, 2> r = load_vec<T, 2>(row + (threadIdx.x & 31) * 2);
+  return make_float2(to_float(r.v[0]), to_float(r.v[1]));
+}
+
+// Stores a lane's two channels, of which `count` exist.
+template <typename T>
+__device__ __forceinline__ void store_pair(T* p, float2 x, int count, bool pairs) {
+  if (pairs) {
+    const float y[2] = {x.x, x.y};
+    if (count > 0) store_vec<T, 2>(p, y);
+  } else {
+    if (count > 0) p[0] = from_float<T>(x.x);
+    if (count > 1) p[1] = from_float<T>(x.y);
+  }
+}
+// Stores a lane's two channels of `rows` rows.
+template <typename T>
+__device__ __forceinline__ void store_rows(T* p, const float2 (&x)[kRows], int64_t dim, int rows, int count, bool pairs) {
+  if (rows == kRows && pairs) {
+    if (count > 0) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i, p += dim) store_pair<T>(p, x[i], 2, true);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i, p += dim)
+      if (i < rows) store_pair<T>(p, x[i], count, pairs);
+  }
+}
+__device__ __forceinline__ float2 load_pair(const float* p, int count) {
+  return make_float2(count > 0 ? p[0] : 0.f, count > 1 ? p[1] : 0.f);
 }
 
 // Rows that no sequence holds, of the channels of this block: those before the first sequence and
 // behind the last one.
-template <typename T, int VEC>
-__device__ __forceinline__ void clear_rest(const ScanArgs& p, T* out, int64_t b, int64_t ch, int part, int parts) {
-  const float zero[VEC] = {};
-  const int warp = part * kWarps + (threadIdx.x >> 5), warps = parts * kWarps;
-  if (ch >= p.dim) return;
+template <typename T>
+__device__ __forceinline__ void clear_rest(const ScanArgs& p, T* out, int64_t b, int count, int part, int parts) {
+  const int warp = part * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = parts * (blockDim.x >> 5);
   if (b == 0) {
     const int64_t first = load_index(p.offsets, 0, p.wide);
-    for (int64_t r = warp; r < first && r < p.tokens; r += warps) store_vec<T, VEC>(out + r * p.dim + ch, zero);
+    for (int64_t r = warp; r < first && r < p.tokens; r += warps) store_pair<T>(out + r * p.dim, make_float2(0.f, 0.f), count, p.pairs);
   }
   if (b == p.batch - 1) {
     const int64_t end = load_index(p.offsets, p.batch, p.wide);
-    for (int64_t r = (end < 0 ? 0 : end) + warp; r < p.tokens; r += warps) store_vec<T, VEC>(out + r * p.dim + ch, zero);
+    for (int64_t r = (end < 0 ? 0 : end) + warp; r < p.tokens; r += warps)
+      store_pair<T>(out + r * p.dim, make_float2(0.f, 0.f), count, p.pairs);
   }
 }
 
-// VEC floats of every lane, in shared memory, lanes side by side.
-template <int VEC>
-struct Lanes {
-  Vec<float, VEC> lane[32];
+// ------------------------------------------------------------------ maps
+// A product of gates stays finite, so that it does not turn a state of 0 into NaN.  (The sums hold what is not
+// a number in the gates: 0 times it is added to them.)
+__device__ __forceinline__ float2 finite(float2 a) {
+  constexpr float kMost = 3.402823466e38f;
+  return make_float2(fminf(fmaxf(a.x, -kMost), kMost), fminf(fmaxf(a.y, -kMost), kMost));
+}
+
+struct Map {  // h -> a h + b, of a lane's two channels
+  float2 a, b;
 };
 
-template <int VEC>
-__device__ __forceinline__ void apply(float (&h)[VEC], const Vec<float, VEC>& A, const Vec<float, VEC>& H) {
-#pragma unroll
-  for (int c = 0; c < VEC; ++c) h[c] = h[c] == 0.f ? H.v[c] : fmaf(A.v[c], h[c], H.v[c]);
-  // (a product of gates that overflowed must not turn a state of 0 into NaN)
+// The maps of a block's warps and of a cluster's blocks, lanes side by side; two sets, used in turn.
+struct Maps {
+  float2 warp_a[2][kMaxWarps][32], warp_b[2][kMaxWarps][32];
+  float2 block_a[2][kMaxCluster][32], block_b[2][kMaxCluster][32];
+};
+
+// Joins the maps of all warps and blocks of the window: `state` goes from before the window to
+// behind it (REVERSE: time runs backwards, from the last block and warp to the first); returns the state this warp's rows
+// start from, and in `at_chunk` the one this warp's chunk starts from.
+template <bool REVERSE>
+__device__ __forceinline__ float2 join_maps(Maps& m, const Map& mine, float2& state, float2& at_chunk, int side,
+                                            const cg::cluster_group& cluster, int part, int parts) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int at = REVERSE ? warps - 1 - warp : warp, chunk = at & ~(kChunkWarps - 1);
+  m.warp_a[side][at][lane] = finite(mine.a);
+  m.warp_b[side][at][lane] = mine.b;
+  __syncthreads();
+  float2 before = state;
+  if (parts > 1) {
+    Map all = {m.warp_a[side][0][lane], m.warp_b[side][0][lane]};
+    for (int j = 1; j < warps; ++j) {
+      const float2 a = m.warp_a[side][j][lane];
+      all.b = fma2(a, all.b, m.warp_b[side][j][lane]);
+      all.a = mul2(a, all.a);
+    }
+    all.a = finite(all.a);
+    const int place = REVERSE ? parts - 1 - part : part;
+    if (warp < parts) {
+      cluster.map_shared_rank(m.block_a[side][place], warp)[lane] = all.a;
+      cluster.map_shared_rank(m.block_b[side][place], warp)[lane] = all.b;
+    }
+    for (int q = warp + warps; q < parts; q += warps) {
+      cluster.map_shared_rank(m.block_a[side][place], q)[lane] = all.a;
+      cluster.map_shared_rank(m.block_b[side][place], q)[lane] = all.b;
+    }
+    cluster.sync();
+    for (int q = 0; q < parts; ++q) {
+      if (q == place) before = state;
+      state = fma2(m.block_a[side][q][lane], state, m.block_b[side][q][lane]);
+    }
+    at_chunk = before;
+    for (int j = 0; j < at; ++j) {
+      before = fma2(m.warp_a[side][j][lane], before, m.warp_b[side][j][lane]);
+      if (j + 1 == chunk) at_chunk = before;
+    }
+  } else {
+    at_chunk = state;
+    for (int j = 0; j < warps; ++j) {
+      if (j == chunk) at_chunk = state;
+      if (j == at) before = state;
+      state = fma2(m.warp_a[side][j][lane], state, m.warp_b[side][j][lane]);
+    }
+  }
+  return before;
 }
 
-template <typename T, typename A, int GATE, int VEC>
-__global__ void __launch_bounds__(kWarps * 32)
+// ------------------------------------------------------------------ forward
+template <typename T, typename A, int GATE>
+__global__ void __launch_bounds__(kMaxWarps * 32, kForwardBlocks)
 linear_scan_kernel(const ScanArgs p) {
-  __shared__ Lanes<VEC> warp_a[2][kWarps], warp_h[2][kWarps];
-  __shared__ Lanes<VEC> block_a[2][kMaxCluster], block_h[2][kMaxCluster];
+  __shared__ Maps maps;
+  extern __shared__ __align__(16) unsigned char ring[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t group = blockIdx.x / parts;
   const int64_t b     = group / p.columns;
-  const int64_t ch    = (group % p.columns) * (32 * VEC) + lane * VEC;
-  const bool in_dim   = ch < p.dim;
-  const Sequence s    = sequence_of(p, b);
-  const A* a = static_cast<const A*>(p.a) + s.a + ch;
-  const T* x = static_cast<const T*>(p.x) + s.x + ch;
+  const int64_t first = (group % p.columns) * kWidth, ch = first + lane * 2;
+  const int left = p.dim - first < kWidth ? int(p.dim - first) : kWidth;  // channels of the block
+  const int count = left - lane * 2;                                      // of the lane: above 0, above 1
+  const Sequence s = sequence_of(p, b);
+  const A* a = static_cast<const A*>(p.a) + s.a + first;
+  const T* x = static_cast<const T*>(p.x) + s.x + first;
   T* out     = static_cast<T*>(p.h) + s.out + ch;
 
-  float carry[VEC];  // the state before the current window
-#pragma unroll
-  for (int c = 0; c < VEC; ++c) carry[c] = 0.f;
-  if (p.h0 && in_dim) {
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) carry[c] = p.h0[b * p.dim + ch + c];
-  }
-
+  float2 state = p.h0 ? load_pair(p.h0 + b * p.dim + ch, count) : make_float2(0.f, 0.f);  // before the window
   if (parts > 1) cluster.sync();  // no block writes to another's shared memory before that has begun
-  const int64_t step = int64_t(parts) * kChunk;
-  int64_t row        = int64_t(part) * kChunk + warp * kRows;
-  Vec<A, VEC> next_a[kRows];
-  Vec<T, VEC> next_x[kRows];
-  load_rows<A, VEC>(next_a, a, p.a_row, row, s.length, in_dim);
-  load_rows<T, VEC>(next_x, x, p.x_row, row, s.length, in_dim);
-  int side = 0;
+
+  constexpr int kStage = kRows * kWidth * int(sizeof(A) + sizeof(T));
+  unsigned char* mine  = ring + warp * p.stages * kStage;
+  const int64_t step   = int64_t(parts) * warps * kRows;
+  int64_t row          = (int64_t(part) * warps + warp) * kRows;  // of this warp in the window
+  auto fetch = [&](int64_t from, int stage) {
+    A* to = reinterpret_cast<A*>(mine + stage * kStage);
+    if (from < s.length) {
+      copy_rows<A>(to, a, p.a_row, from, s.length, left, p.a_piece);
+      copy_rows<T>(reinterpret_cast<T*>(to + kRows * kWidth), x, p.x_row, from, s.length, left, p.x_piece);
+    }
+    copy_commit();
+  };
+  for (int i = 0; i < p.stages; ++i) fetch(row + i * step, i);
+  int side = 0, stage = 0;
   for (int64_t window = 0; window < s.length; window += step, row += step, side ^= 1) {
-    float f[kRows][VEC], u[kRows][VEC];
-    Vec<float, VEC> prod, sum;
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) prod.v[c] = 1.f, sum.v[c] = 0.f;
+    copy_wait(p.stages - 1);
+    __syncwarp();
+    const A* sa = reinterpret_cast<const A*>(mine + stage * kStage);
+    const T* sx = reinterpret_cast<const T*>(sa + kRows * kWidth);
+    const int rows = s.length - row < kRows ? int(s.length - row) : kRows;  // of this warp; may be negative
+    float2 f[kRows], rest[kRows];  // rest: 1 - f, SIGMOID only
+    Map map = {make_float2(1.f, 1.f), make_float2(0.f, 0.f)};
+    auto input_at = [&](int i) {  // u of row i
+      const float2 gx = pair_at<T>(sx + i * kWidth);
+      if constexpr (GATE == TCU_GATE_SIGMOID) return mul2(rest[i], gx);
+      return gx;
+    };
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const bool inside = row + i < s.length;  // rows behind the end: the identity
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        float unused;
-        gate_of<GATE>(to_float(next_a[i].v[c]), to_float(next_x[i].v[c]), f[i][c], u[i][c], unused);
-        f[i][c] = inside ? f[i][c] : 1.f;
-        u[i][c] = inside ? u[i][c] : 0.f;
-        sum.v[c] = fmaf(f[i][c], sum.v[c], u[i][c]);
-        prod.v[c] *= f[i][c];
-      }
+      const float2 ga = pair_at<A>(sa + i * kWidth);
+      gate_of<GATE>(ga.x, f[i].x, rest[i].x);
+      gate_of<GATE>(ga.y, f[i].y, rest[i].y);
     }
-    if (window + step < s.length) {
-      load_rows<A, VEC>(next_a, a, p.a_row, row + step, s.length, in_dim);
-      load_rows<T, VEC>(next_x, x, p.x_row, row + step, s.length, in_dim);
-    }
-    warp_a[side][warp].lane[lane] = prod;
-    warp_h[side][warp].lane[lane] = sum;
-    __syncthreads();
-    float h[VEC];  // becomes the state before this warp's rows
-    if (parts > 1) {
-      // this block's map to all blocks of the cluster: warp r writes to block r
-      Vec<float, VEC> A_ = warp_a[side][0].lane[lane];
-      Vec<float, VEC> H_ = warp_h[side][0].lane[lane];
+    if (rows == kRows) {
 #pragma unroll
-      for (int j = 1; j < kWarps; ++j) {
-        const Vec<float, VEC> aj = warp_a[side][j].lane[lane], hj = warp_h[side][j].lane[lane];
-        apply<VEC>(H_.v, aj, hj);
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) A_.v[c] *= aj.v[c];
-      }
-      if (warp < parts) {
-        cluster.map_shared_rank(&block_a[side][part], warp)->lane[lane] = A_;
-        cluster.map_shared_rank(&block_h[side][part], warp)->lane[lane] = H_;
-      }
-      cluster.sync();
-      float before[VEC];
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) before[c] = carry[c];
-      for (int q = 0; q < parts; ++q) {
-        if (q == part) {
-#pragma unroll
-          for (int c = 0; c < VEC; ++c) before[c] = carry[c];
-        }
-        apply<VEC>(carry, block_a[side][q].lane[lane], block_h[side][q].lane[lane]);
-      }
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) h[c] = before[c];
+      for (int i = 0; i < kRows; ++i) map.b = fma2(f[i], map.b, input_at(i)), map.a = mul2(map.a, f[i]);
     } else {
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) h[c] = carry[c];
-#pragma unroll
-      for (int j = 0; j < kWarps; ++j)
-        apply<VEC>(carry, warp_a[side][j].lane[lane], warp_h[side][j].lane[lane]);
+      for (int i = 0; i < kRows; ++i)  // (rows behind the end: the identity)
+        if (i < rows) map.b = fma2(f[i], map.b, input_at(i)), map.a = mul2(map.a, f[i]);
     }
-    const int64_t chunk = window / kChunk + part;
-    if (p.states && warp == 0 && in_dim && chunk * kChunk < s.length)
-      store_vec<float, VEC>(p.states + (s.chunk + chunk) * p.dim + ch, h);
-    for (int j = 0; j < warp; ++j)
-      apply<VEC>(h, warp_a[side][j].lane[lane], warp_h[side][j].lane[lane]);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) h[c] = fmaf(f[i][c], h[c], u[i][c]);
-      if (in_dim && row + i < s.length) store_vec<T, VEC>(out + (row + i) * p.dim, h);
+    float2 at_chunk;
+    float2 h = join_maps<false>(maps, map, state, at_chunk, side, cluster, part, parts);
+    if (p.states && warp % kChunkWarps == 0 && rows > 0) {
+      float* st = p.states + (s.chunk + row / kChunk) * p.dim + ch;
+      if (count > 0) st[0] = at_chunk.x;
+      if (count > 1) st[1] = at_chunk.y;
     }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) f[i] = h = fma2(f[i], h, input_at(i));
+    store_rows<T>(out + row * p.dim, f, p.dim, rows, count, p.pairs);
+    __syncwarp();  // every lane has read the stage
+    fetch(row + p.stages * step, stage);
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
   }
-  if (p.clear_rest) clear_rest<T, VEC>(p, static_cast<T*>(p.h), b, ch, part, parts);
-  if (p.last && part == 0 && warp == 0 && in_dim) store_vec<float, VEC>(p.last + b * p.dim + ch, carry);
+  if (p.clear_rest) clear_rest<T>(p, static_cast<T*>(p.h) + ch, b, count, part, parts);
+  if (p.last && part == 0 && warp == 0) {
+    float* last = p.last + b * p.dim + ch;
+    if (count > 0) last[0] = state.x;
+    if (count > 1) last[1] = state.y;
+  }
 }
 
-template <typename T, typename A, int GATE, int VEC>
-__global__ void __launch_bounds__(kWarps * 32)
+// ------------------------------------------------------------------ backward
+template <typename T, typename A, int GATE>
+__global__ void __launch_bounds__(kMaxWarps * 32, kBackwardBlocks)
 linear_scan_backward_kernel(const ScanArgs p) {
-  __shared__ Lanes<VEC> warp_a[2][kWarps], warp_h[2][kWarps], warp_g[2][kWarps];
-  __shared__ Lanes<VEC> block_a[2][kMaxCluster], block_g[2][kMaxCluster];
+  __shared__ Maps maps;
+  __shared__ float2 forward_a[2][kMaxWarps][32], forward_b[2][kMaxWarps][32];
+  extern __shared__ __align__(16) unsigned char ring[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t group = blockIdx.x / parts;
   const int64_t b     = group / p.columns;
-  const int64_t ch    = (group % p.columns) * (32 * VEC) + lane * VEC;
-  const bool in_dim   = ch < p.dim;
-  const Sequence s    = sequence_of(p, b);
-  const A* a  = static_cast<const A*>(p.a) + s.a + ch;
-  const T* x  = static_cast<const T*>(p.x) + s.x + ch;
-  const T* dy = static_cast<const T*>(p.dh) + s.dh + ch;
+  const int64_t first = (group % p.columns) * kWidth, ch = first + lane * 2;
+  const int left = p.dim - first < kWidth ? int(p.dim - first) : kWidth;
+  const int count = left - lane * 2;
+  const Sequence s = sequence_of(p, b);
+  const A* a  = static_cast<const A*>(p.a) + s.a + first;
+  const T* x  = static_cast<const T*>(p.x) + s.x + first;
+  const T* dy = static_cast<const T*>(p.dh) + s.dh + first;
   A* da       = static_cast<A*>(p.da) + s.out + ch;
   T* dx       = static_cast<T*>(p.dx) + s.out + ch;
-
-  float carry[VEC];  // what the rows behind the current window pass back
-#pragma unroll
-  for (int c = 0; c < VEC; ++c) carry[c] = 0.f;
-  if (p.dlast && in_dim) {
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) carry[c] = p.dlast[b * p.dim + ch + c];
-  }
-
-  if (parts > 1) cluster.sync();
-  const int64_t step    = int64_t(parts) * kChunk;
-  const int64_t windows = (s.length + step - 1) / step;
-  int64_t row           = (windows - 1) * step + int64_t(part) * kChunk + warp * kRows;
-  Vec<A, VEC> next_a[kRows];
-  Vec<T, VEC> next_x[kRows], next_d[kRows];
   const bool has_dy = p.dh != nullptr;
-  if (windows > 0) {
-    load_rows<A, VEC>(next_a, a, p.a_row, row, s.length, in_dim);
-    load_rows<T, VEC>(next_x, x, p.x_row, row, s.length, in_dim);
-    load_rows<T, VEC>(next_d, dy, p.dh_row, row, s.length, in_dim && has_dy);
-  }
-  int side = 0;
-  for (int64_t window = (windows - 1) * step; window >= 0; window -= step, row -= step, side ^= 1) {
-    const int64_t chunk = window / kChunk + part;
-    float h[VEC];  // the state before this chunk
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) h[c] = 0.f;
-    if (in_dim && chunk * kChunk < s.length) {
-      const Vec<float, VEC> st = load_vec<float, VEC>(p.states + (s.chunk + chunk) * p.dim + ch);
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) h[c] = st.v[c];
+
+  float2 state = p.dlast ? load_pair(p.dlast + b * p.dim + ch, count) : make_float2(0.f, 0.f);  // passed back by the rows behind
+  if (parts > 1) cluster.sync();
+
+  constexpr int kStage  = kRows * kWidth * int(sizeof(A) + 2 * sizeof(T));
+  unsigned char* mine   = ring + warp * p.stages * kStage;
+  const int64_t step    = int64_t(parts) * warps * kRows;
+  const int64_t windows = (s.length + step - 1) / step;
+  int64_t row           = (windows - 1) * step + (int64_t(part) * warps + warp) * kRows;
+  auto fetch = [&](int64_t from, int stage) {
+    A* to = reinterpret_cast<A*>(mine + stage * kStage);
+    T* tx = reinterpret_cast<T*>(to + kRows * kWidth);
+    if (from >= 0 && from < s.length) {
+      copy_rows<A>(to, a, p.a_row, from, s.length, left, p.a_piece);
+      copy_rows<T>(tx, x, p.x_row, from, s.length, left, p.x_piece);
+      if (has_dy) copy_rows<T>(tx + kRows * kWidth, dy, p.dh_row, from, s.length, left, p.dh_piece);
     }
-    float f[kRows][VEC], u[kRows][VEC], rest[kRows][VEC], d[kRows][VEC];
-    Vec<float, VEC> prod, sum, back;
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) prod.v[c] = 1.f, sum.v[c] = 0.f, back.v[c] = 0.f;
+    copy_commit();
+  };
+  for (int i = 0; i < p.stages; ++i) fetch(row - i * step, i);
+  int side = 0, stage = 0;
+  for (int64_t window = 0; window < windows; ++window, row -= step, side ^= 1) {
+    const int rows = s.length - row < kRows ? int(s.length - row) : kRows;
+    float2 h = make_float2(0.f, 0.f);  // the state before this warp's chunk of rows
+    if (rows > 0) h = load_pair(p.states + (s.chunk + row / kChunk) * p.dim + ch, count);
+    copy_wait(p.stages - 1);
+    __syncwarp();
+    const A* sa = reinterpret_cast<const A*>(mine + stage * kStage);
+    const T* sx = reinterpret_cast<const T*>(sa + kRows * kWidth);
+    const T* sd = sx + kRows * kWidth;
+    float2 f[kRows], rest[kRows];  // rest: 1 - f, SIGMOID only
+    Map forward = {make_float2(1.f, 1.f), make_float2(0.f, 0.f)}, back = forward;
+    auto gradient_at = [&](int i) {  // dy of row i
+      return has_dy ? pair_at<T>(sd + i * kWidth) : make_float2(0.f, 0.f);
+    };
+    auto input_at = [&](int i) {  // u of row i
+      const float2 gx = pair_at<T>(sx + i * kWidth);
+      if constexpr (GATE == TCU_GATE_SIGMOID) return mul2(rest[i], gx);
+      return gx;
+    };
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const bool inside = row + i < s.length;
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        gate_of<GATE>(to_float(next_a[i].v[c]), to_float(next_x[i].v[c]), f[i][c], u[i][c], rest[i][c]);
-        f[i][c] = inside ? f[i][c] : 1.f;
-        u[i][c] = inside ? u[i][c] : 0.f;
-        d[i][c] = to_float(next_d[i].v[c]);
-        sum.v[c] = fmaf(f[i][c], sum.v[c], u[i][c]);
-        prod.v[c] *= f[i][c];
-      }
+      const float2 ga = pair_at<A>(sa + i * kWidth);
+      gate_of<GATE>(ga.x, f[i].x, rest[i].x);
+      gate_of<GATE>(ga.y, f[i].y, rest[i].y);
     }
+    auto first_pass = [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
-    for (int i = kRows - 1; i >= 0; --i) {
+      for (int i = 0; i < kRows; ++i)
+        if (kWhole || i < rows) forward.b = fma2(f[i], forward.b, input_at(i)), forward.a = mul2(forward.a, f[i]);
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) back.v[c] = f[i][c] * (d[i][c] + back.v[c]);
-    }
-    float xs[kRows][VEC];  // only SIGMOID needs x again
-    if constexpr (GATE == TCU_GATE_SIGMOID) {
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) xs[i][c] = to_float(next_x[i].v[c]);
-      }
-    }
-    if (window > 0) {
-      load_rows<A, VEC>(next_a, a, p.a_row, row - step, s.length, in_dim);
-      load_rows<T, VEC>(next_x, x, p.x_row, row - step, s.length, in_dim);
-      load_rows<T, VEC>(next_d, dy, p.dh_row, row - step, s.length, in_dim && has_dy);
-    }
-    warp_a[side][warp].lane[lane] = prod;
-    warp_h[side][warp].lane[lane] = sum;
-    warp_g[side][warp].lane[lane] = back;
-    __syncthreads();
-    float g[VEC];  // becomes what the rows behind this warp's pass back
-    if (parts > 1) {
-      Vec<float, VEC> A_ = warp_a[side][kWarps - 1].lane[lane];
-      Vec<float, VEC> G_ = warp_g[side][kWarps - 1].lane[lane];
-#pragma unroll
-      for (int j = kWarps - 2; j >= 0; --j) {
-        const Vec<float, VEC> aj = warp_a[side][j].lane[lane], gj = warp_g[side][j].lane[lane];
-        apply<VEC>(G_.v, aj, gj);
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) A_.v[c] *= aj.v[c];
-      }
-      if (warp < parts) {
-        cluster.map_shared_rank(&block_a[side][part], warp)->lane[lane] = A_;
-        cluster.map_shared_rank(&block_g[side][part], warp)->lane[lane] = G_;
-      }
-      cluster.sync();
-      float behind[VEC];
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) behind[c] = carry[c];
-      for (int q = parts - 1; q >= 0; --q) {
-        if (q == part) {
-#pragma unroll
-          for (int c = 0; c < VEC; ++c) behind[c] = carry[c];
-        }
-        apply<VEC>(carry, block_a[side][q].lane[lane], block_g[side][q].lane[lane]);
-      }
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) g[c] = behind[c];
-    } else {
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) g[c] = carry[c];
-#pragma unroll
-      for (int j = kWarps - 1; j >= 0; --j)
-        apply<VEC>(carry, warp_a[side][j].lane[lane], warp_g[side][j].lane[lane]);
-    }
-    for (int j = kWarps - 1; j > warp; --j)
-      apply<VEC>(g, warp_a[side][j].lane[lane], warp_g[side][j].lane[lane]);
-    for (int j = 0; j < warp; ++j)
-      apply<VEC>(h, warp_a[side][j].lane[lane], warp_h[side][j].lane[lane]);
-    float before[kRows][VEC];
+      for (int i = kRows - 1; i >= 0; --i)
+        if (kWhole || i < rows) back.b = mul2(f[i], add2(gradient_at(i), back.b));
+    };
+    if (rows == kRows)
+      first_pass(std::true_type{});
+    else
+      first_pass(std::false_type{});
+    back.a = forward.a;
+    forward_a[side][warp][lane] = finite(forward.a);
+    forward_b[side][warp][lane] = forward.b;
+    float2 unused;
+    float2 g = join_maps<true>(maps, back, state, unused, side, cluster, part, parts);
+    for (int j = warp & ~(kChunkWarps - 1); j < warp; ++j) h = fma2(forward_a[side][j][lane], h, forward_b[side][j][lane]);
+    float2 before[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        before[i][c] = h[c];
-        h[c]         = fmaf(f[i][c], h[c], u[i][c]);
-      }
+      before[i] = h;
+      h         = fma2(f[i], h, input_at(i));
     }
+    // before becomes da, f becomes dx
+    auto second_pass = [&](auto whole) {
 #pragma unroll
-    for (int i = kRows - 1; i >= 0; --i) {
-      float ga[VEC], gx[VEC];
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        const float dh = d[i][c] + g[c];
+      for (int i = kRows - 1; i >= 0; --i) {
+        if (!decltype(whole)::value && i >= rows) continue;
+        const float2 dh = add2(gradient_at(i), g), fi = f[i];
+        g = mul2(fi, dh);
         if constexpr (GATE == TCU_GATE_SIGMOID) {
-          ga[c] = dh * (before[i][c] - xs[i][c]) * f[i][c] * rest[i][c];
-          gx[c] = dh * rest[i][c];
+          const float2 v = pair_at<T>(sx + i * kWidth);
+          before[i] = mul2(mul2(dh, add2(before[i], make_float2(-v.x, -v.y))), mul2(fi, rest[i]));
+          f[i]      = mul2(dh, rest[i]);
         } else {
-          ga[c] = GATE == TCU_GATE_LOG ? dh * before[i][c] * f[i][c] : dh * before[i][c];
-          gx[c] = dh;
+          before[i] = mul2(GATE == TCU_GATE_LOG ? g : dh, before[i]);
+          f[i]      = dh;
         }
-        g[c] = f[i][c] * dh;
       }
-      if (in_dim && row + i < s.length) {
-        store_vec<A, VEC>(da + (row + i) * p.dim, ga);
-        store_vec<T, VEC>(dx + (row + i) * p.dim, gx);
-      }
-    }
+    };
+    if (rows == kRows)
+      second_pass(std::true_type{});
+    else
+      second_pass(std::false_type{});
+    store_rows<A>(da + row * p.dim, before, p.dim, rows, count, p.pairs);
+    store_rows<T>(dx + row * p.dim, f, p.dim, rows, count, p.pairs);
+    __syncwarp();
+    fetch(row - p.stages * step, stage);
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
   }
   if (p.clear_rest) {
-    clear_rest<A, VEC>(p, static_cast<A*>(p.da), b, ch, part, parts);
-    clear_rest<T, VEC>(p, static_cast<T*>(p.dx), b, ch, part, parts);
+    clear_rest<A>(p, static_cast<A*>(p.da) + ch, b, count, part, parts);
+    clear_rest<T>(p, static_cast<T*>(p.dx) + ch, b, count, part, parts);
   }
-  if (p.dh0 && part == 0 && warp == 0 && in_dim) store_vec<float, VEC>(p.dh0 + b * p.dim + ch, carry);
+  if (p.dh0 && part == 0 && warp == 0) {
+    float* dh0 = p.dh0 + b * p.dim + ch;
+    if (count > 0) dh0[0] = state.x;
+    if (count > 1) dh0[1] = state.y;
+  }
 }
 
 struct StepArgs {
@@ -448,9 +543,9 @@ linear_scan_step_kernel(const StepArgs p) {
   float h[VEC];
 #pragma unroll
   for (int c = 0; c < VEC; ++c) {
-    float f, u, unused;
-    gate_of<GATE>(to_float(a.v[c]), to_float(x.v[c]), f, u, unused);
-    h[c] = fmaf(f, before.v[c], u);
+    float f, rest = 1.f;
+    gate_of<GATE>(to_float(a.v[c]), f, rest);
+    h[c] = fmaf(f, before.v[c], rest * to_float(x.v[c]));
   }
   store_vec<float, VEC>(state, h);
   store_vec<T, VEC>(static_cast<T*>(p.h) + b * p.dim + ch, h);
@@ -483,23 +578,48 @@ int check_types(int64_t type, int64_t a_type, int64_t gate) {
   return TCU_OK;
 }
 
-// Blocks per sequence and column of channels: as many as it takes to give every SM two blocks, if
-// the sequences have the rows for them.
-int cluster_size(int64_t blocks, int64_t tokens_each, int sms) {
-  int parts = 1;
-  while (parts < kMaxCluster && blocks * parts < 2 * sms && tokens_each > int64_t(parts) * kChunk) parts *= 2;
-  return parts;
+// How many bytes of rows that begin at p can be copied at a time.
+int piece_of(const void* p, size_t elem, int64_t dim, int64_t batch_stride, int64_t row_stride) {
+  auto fits = [&](int64_t bytes) {
+    return aligned(p, bytes) && dim * int64_t(elem) % bytes == 0 && batch_stride * int64_t(elem) % bytes == 0 &&
+           row_stride * int64_t(elem) % bytes == 0;
+  };
+  return fits(16) ? 16 : fits(4) ? 4 : int(elem);
 }
 
-cudaError_t launch_clusters(void (*kernel)(const ScanArgs), ScanArgs args, int vec, int sms, cudaStream_t st) {
-  args.columns         = int((args.dim + 32 * vec - 1) / (32 * vec));
+constexpr int kSharedPerSm = 220 << 10;
+
+// Warps per block and blocks per cluster: as many as it takes to give every SM kWarpsWanted warps, if the
+// sequences have the rows for them; blocks of 8 warps before clusters, which have to meet.  Stages: what then fits.
+constexpr int kWarpsWanted = 8;
+
+template <void (*Kernel)(const ScanArgs)>
+cudaError_t launch_clusters(ScanArgs args, int stage_bytes, int static_bytes, int sms, cudaStream_t st) {
+  args.columns         = int((args.dim + kWidth - 1) / kWidth);
   const int64_t groups = args.batch * args.columns;
   const int64_t each   = args.offsets ? 2 * args.tokens / args.batch : args.tokens;
-  const int parts      = cluster_size(groups, each, sms);
+  int warps = kChunkWarps, parts = 1;
+  auto more = [&] { return groups * parts * warps < int64_t(sms) * kWarpsWanted && each > int64_t(parts) * warps * kRows; };
+  if (more()) warps = kMaxWarps;
+  while (parts < kMaxCluster && more()) parts *= 2;
   if (groups * parts > int64_t(0x7fffffff)) return cudaErrorInvalidConfiguration;
+  const int64_t per_sm = (groups * parts + sms - 1) / sms;  // blocks that there are for an SM
+  int stages = 2;
+  while (stages < kMaxStages && per_sm * ((stages + 1) * warps * stage_bytes + static_bytes) <= kSharedPerSm) ++stages;
+  args.stages     = stages;
+  const int bytes = stages * warps * stage_bytes;
+  static bool configured[kMaxDevices];
+  const int dev = current_device();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedPerSm - static_bytes);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim            = dim3(unsigned(groups * parts));
-  cfg.blockDim           = dim3(kWarps * 32);
+  cfg.blockDim           = dim3(warps * 32);
+  cfg.dynamicSmemBytes   = bytes;
   cfg.stream             = st;
   cudaLaunchAttribute attr[1];
   attr[0].id                 = cudaLaunchAttributeClusterDimension;
@@ -508,7 +628,7 @@ cudaError_t launch_clusters(void (*kernel)(const ScanArgs), ScanArgs args, int v
   attr[0].val.clusterDim.z   = 1;
   cfg.attrs    = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args);
+  return cudaLaunchKernelEx(&cfg, Kernel, args);
 }
 
 bool bad_sizes(int64_t batch, int64_t tokens, int64_t dim) {
@@ -547,20 +667,14 @@ int tcu_linear_scan(const tcu_linear_scan_args* g, void* stream) {
   p.x_batch = g->offsets ? 0 : g->x_batch_stride, p.x_row = g->x_row_stride;
   p.wide = g->offsets_are_64bit != 0;
   p.clear_rest = g->offsets && g->clear_rest;
-  auto fits = [&](int v) {
-    return p.dim % v == 0 && vector_rows(p.a, ea, p.a_batch, p.a_row, v) && vector_rows(p.x, e, p.x_batch, p.x_row, v) &&
-           aligned(p.h, e * v) && aligned(p.last, 4 * v) && aligned(p.states, 4 * v);
-  };
+  p.a_piece = piece_of(p.a, ea, p.dim, p.a_batch, p.a_row), p.x_piece = piece_of(p.x, e, p.dim, p.x_batch, p.x_row);
+  p.pairs   = p.dim % 2 == 0 && aligned(p.h, 2 * e);
   const cudaError_t err = for_types(g->type, g->a_type, g->gate, [&](auto t, auto a, auto gate) {
     using T = decltype(t);
     using A = decltype(a);
-    constexpr int G = decltype(gate)::value;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if constexpr (sizeof(T) == 2) {
-      if (fits(4)) return launch_clusters(linear_scan_kernel<T, A, G, 4>, p, 4, sms, st);
-    }
-    if (fits(2)) return launch_clusters(linear_scan_kernel<T, A, G, 2>, p, 2, sms, st);
-    return launch_clusters(linear_scan_kernel<T, A, G, 1>, p, 1, sms, st);
+    return launch_clusters<linear_scan_kernel<T, A, decltype(gate)::value>>(
+        p, kRows * kWidth * int(sizeof(A) + sizeof(T)),
+                           sizeof(Maps), sms, static_cast<cudaStream_t>(stream));
   });
   return err == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
 }
@@ -587,18 +701,15 @@ int tcu_linear_scan_backward(const tcu_linear_scan_backward_args* g, void* strea
   p.dh_batch = g->offsets ? 0 : g->dh_batch_stride, p.dh_row = g->dh_row_stride;
   p.wide = g->offsets_are_64bit != 0;
   p.clear_rest = g->offsets && g->clear_rest;
-  auto fits = [&](int v) {
-    return p.dim % v == 0 && vector_rows(p.a, ea, p.a_batch, p.a_row, v) && vector_rows(p.x, e, p.x_batch, p.x_row, v) &&
-           vector_rows(p.dh, e, p.dh_batch, p.dh_row, v) && aligned(p.da, ea * v) && aligned(p.dx, e * v) &&
-           aligned(p.dh0, 4 * v) && aligned(p.states, 4 * v);
-  };
+  p.a_piece = piece_of(p.a, ea, p.dim, p.a_batch, p.a_row), p.x_piece = piece_of(p.x, e, p.dim, p.x_batch, p.x_row);
+  p.dh_piece = piece_of(p.dh, e, p.dim, p.dh_batch, p.dh_row);
+  p.pairs    = p.dim % 2 == 0 && aligned(p.da, 2 * ea) && aligned(p.dx, 2 * e);
   const cudaError_t err = for_types(g->type, g->a_type, g->gate, [&](auto t, auto a, auto gate) {
     using T = decltype(t);
     using A = decltype(a);
-    constexpr int G = decltype(gate)::value;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (fits(2)) return launch_clusters(linear_scan_backward_kernel<T, A, G, 2>, p, 2, sms, st);
-    return launch_clusters(linear_scan_backward_kernel<T, A, G, 1>, p, 1, sms, st);
+    return launch_clusters<linear_scan_backward_kernel<T, A, decltype(gate)::value>>(
+        p, kRows * kWidth * int(sizeof(A) + 2 * sizeof(T)), sizeof(Maps) + 4 * kMaxWarps * 32 * 8, sms,
+                           static_cast<cudaStream_t>(stream));
   });
   return err == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
 }

@@ -67,6 +67,44 @@ __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, bool wid
   return wide ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
 }
 
+// ------------------------------------------------------------------ functions
+constexpr float kLog2E = 1.44269504088896341f;
+
+// 2^x within 2 ulp; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / x within 1 ulp.
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ------------------------------------------------------------------ pairs
+// sm_100 adds, multiplies and multiply-adds two floats with one instruction.
+#define TCU_PAIR_OP(name, op)                                                                   \
+  __device__ __forceinline__ float2 name(float2 a, float2 b) {                                  \
+    float2 r;                                                                                   \
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"           \
+        op " z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"                                             \
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));                       \
+    return r;                                                                                   \
+  }
+TCU_PAIR_OP(add2, "add.rn.f32x2")
+TCU_PAIR_OP(mul2, "mul.rn.f32x2")
+#undef TCU_PAIR_OP
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // ------------------------------------------------------------------ reductions
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll

@@ -30,7 +30,6 @@ constexpr int kMaxThreads = 256;
 constexpr int kBlocksPerSm = 4;
 constexpr int kMaxWarps   = kMaxThreads / 32;
 constexpr int kUnroll     = 4;
-constexpr float kLog2E    = 1.44269504088896341f;
 constexpr float kLn2      = 0.693147180559945309f;
 // 2^this is 0 (subnormal results are: a probability below 2^-126 of the sum counts as none); stands for
 // -inf, which 0 * -inf would turn into NaN.
@@ -46,12 +45,6 @@ struct LogprobArgs {
   int top;
   bool wide;
 };
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // The larger of two, NaN if one is.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -70,28 +63,6 @@ __device__ __forceinline__ float value_of(uint32_t o) {
   if (o == 0xffffffffu) return __uint_as_float(0x7fffffffu);
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-
-// ------------------------------------------------------------------ pairs
-// sm_100 adds, multiplies and multiply-adds two floats with one instruction.
-#define TCU_PAIR_OP(name, op)                                                                   \
-  __device__ __forceinline__ float2 name(float2 a, float2 b) {                                  \
-    float2 r;                                                                                   \
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"           \
-        op " z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"                                             \
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));                       \
-    return r;                                                                                   \
-  }
-TCU_PAIR_OP(add2, "add.rn.f32x2")
-TCU_PAIR_OP(mul2, "mul.rn.f32x2")
-#undef TCU_PAIR_OP
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // ------------------------------------------------------------------ rows
 // 16 bytes of logits: kVec<T> elements, kVec<T> / 2 pairs.

@@ -26,6 +26,9 @@ def assert_within(got, want, bound, what):
 # Roundings of one step of the recurrence: the gate (expf and the reciprocal 2 ulp = 4 u each, an
 # addition, a product), 1 - f times x, the product of gates and the fused multiply-add: 12.
 STEP = 12 * U
+# An exponential below float32's smallest normal number, 2^-126, counts as 0: a gate is off by less than that, and
+# what it multiplies by less than that times its size.
+FLUSH = 2.0 ** -126
 
 
 def gates(gate, a, x):
@@ -52,7 +55,8 @@ def linear_scan(gate, a, x, h0, dh=None, dlast=None):
     got = {}
     h = recur(f, u, h0)
     size = recur(f.abs(), u.abs(), h0.abs())          # what the absolute values add up to
-    off = recur(f.abs(), STEP * size, torch.zeros_like(h0))  # each step's roundings, carried on
+    flush = FLUSH * torch.cat([h0.abs()[None], size[:-1]])[:n]
+    off = recur(f.abs(), STEP * size + flush, torch.zeros_like(h0))  # each step's roundings, carried on
     got["h"] = (h, off)
     got["last"] = (h[-1], off[-1]) if n else (h0, torch.zeros_like(h0))
     if dh is None:
@@ -61,20 +65,21 @@ def linear_scan(gate, a, x, h0, dh=None, dlast=None):
     ahead = torch.cat([f[1:], torch.ones_like(f[:1])])[:n]
     g = recur(ahead.flip(0), dh.flip(0), dlast).flip(0) if n else dh
     gsize = recur(ahead.abs().flip(0), dh.abs().flip(0), dlast.abs()).flip(0) if n else dh
-    goff = recur(ahead.abs().flip(0), STEP * gsize.flip(0), torch.zeros_like(dlast)).flip(0) if n else dh
+    gflush = FLUSH * torch.cat([gsize[1:], dlast.abs()[None]])[:n]
+    goff = recur(ahead.abs().flip(0), (STEP * gsize + gflush).flip(0), torch.zeros_like(dlast)).flip(0) if n else dh
     before = torch.cat([h0[None], h[:-1]])[:n]
     bsize = torch.cat([h0.abs()[None], size[:-1]])[:n]
     boff = torch.cat([torch.zeros_like(h0)[None], off[:-1]])[:n]
     if gate == "sigmoid":
         slope = f * rest
         got["da"] = (g * (before - x) * slope,
-                     ((goff + STEP * g.abs()) * (before - x).abs() + g.abs() * (boff + STEP * (bsize + x.abs()))) * slope)
-        got["dx"] = (g * rest, (goff + STEP * g.abs()) * rest)
+                     ((goff + STEP * g.abs()) * (before - x).abs() + g.abs() * (boff + STEP * (bsize + x.abs()))) * slope + FLUSH * gsize * (bsize + x.abs()))
+        got["dx"] = (g * rest, (goff + STEP * g.abs()) * rest + FLUSH * gsize)
     else:
         slope = f if gate == "log" else torch.ones_like(f)
-        got["da"] = (g * before * slope, ((goff + STEP * g.abs()) * before.abs() + g.abs() * (boff + STEP * bsize)) * slope.abs())
+        got["da"] = (g * before * slope, ((goff + STEP * g.abs()) * before.abs() + g.abs() * (boff + STEP * bsize)) * slope.abs() + FLUSH * gsize * bsize)
         got["dx"] = (g, goff)
-    got["dh0"] = (f[0] * g[0], (f[0] * goff[0]).abs() + STEP * gsize[0] * f[0].abs()) if n else (dlast, torch.zeros_like(dlast))
+    got["dh0"] = (f[0] * g[0], (f[0] * goff[0]).abs() + STEP * gsize[0] * f[0].abs() + FLUSH * gsize[0]) if n else (dlast, torch.zeros_like(dlast))
     return got
 
 
