@@ -339,7 +339,7 @@ typedef enum { TCU_TYPE_F16 = 0, TCU_TYPE_F32 = 1, TCU_TYPE_BF16 = 2 } tcu_type;
  * h0, last: batch x dim floats; last (may be h0) receives the state behind
  * each sequence's last row, h0's if the sequence is empty.
  * states: NULL, or tcu_linear_scan_states_rows() x dim floats that
- * tcu_linear_scan_backward() wants (the state before every 64th row).
+ * tcu_linear_scan_backward() wants (the state before every 16th row).
  */
 typedef enum { TCU_GATE_DECAY = 0, TCU_GATE_LOG = 1, TCU_GATE_SIGMOID = 2 } tcu_gate;
 

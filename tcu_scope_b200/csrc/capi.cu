@@ -815,7 +815,8 @@ int tcu_device_error(unsigned int* bits, int clear) {
   if (tcu_error_word_linear_scan(&c, clear) != TCU_OK) return TCU_ERR_CUDA;
   if (tcu_error_word_token_logprobs(&d, clear) != TCU_OK) return TCU_ERR_CUDA;
   if (bits) *bits = a | b | c | d;
-  return (a | b) ? TCU_ERR_TIMEOUT : (c | d) ? TCU_ERR_INDEX : TCU_OK;
+  const unsigned int all = a | b | c | d;
+  return (all & 7u) ? TCU_ERR_TIMEOUT : all ? TCU_ERR_INDEX : TCU_OK;
 }
 
 int tcu_test_set_wait_limits(unsigned barrier_attempts, unsigned status_polls, unsigned flag_polls,

@@ -1,23 +1,22 @@
 // Gated linear recurrence h_t = f_t h_{t-1} + u_t along time, channel by channel, and its gradient.
 //
-// The step h -> f h + u is a linear map, and maps compose: (A2, H2) after (A1, H1) is
-// (A2 A1, A2 H1 + H2).  So time is cut into pieces whose maps are computed independently, and
-// only the maps are passed along:
-//   - a warp takes 16 consecutive rows of 64 channels, two channels a lane, and computes their map;
-//   - the warps of a block take consecutive rows (64 with 4 warps) and exchange maps in shared memory;
-//   - the P blocks of a cluster take consecutive rows of the same channels (a window) and
-//     exchange maps in each other's shared memory;
-//   - the cluster goes through its sequence window by window, the state in registers.
-// Every element is read from and written to memory once.  All maps are joined in the order of time, so the
-// result does not depend on timing.
+// A warp takes 64 channels of a sequence, two channels a lane, 32 rows at a time (a window).  It copies its rows into a
+// ring of its own in shared memory (cp.async, 16 bytes a lane), some windows ahead, so it waits for nothing
+// but its own copies; the state stays in registers.  One such warp moves 38 bytes a nanosecond, and one
+// or two on every SM use up the memory's 44: that is all there is to do where sequences and columns make a
+// warp for every SM.
 //
-// Backwards, with g_t = f_t dh_t passing from row t to row t-1 (dh_t = dy_t + g_{t+1}) the same
-// holds with time reversed; h_{t-1} is recomputed from the state before every 64th row, which the
-// forward pass leaves behind (one row of floats for 64 rows of elements).
+// Where they do not (few sequences, few channels), time is cut as well.  The step h -> f h + u is a linear map, and
+// maps compose: (A2, H2) after (A1, H1) is (A2 A1, A2 H1 + H2).  The warps of a block, and the P blocks of a cluster, take
+// consecutive windows of the same channels, each computes the map of its 16 rows, all exchange the maps in shared memory,
+// each joins those before its own to the state, and then goes through its rows (still in shared memory)
+// once more.  All maps are joined in the order of time, so the result does not depend on timing.
 //
-// Bound by HBM: 3 arrays forward, 5 backward.  Each warp copies its rows into a ring of its own in shared memory
-// (cp.async, 16 bytes a lane), some windows ahead: nothing but its own copies is waited for, and the
-// registers hold the gates of the current window only.
+// Backwards, with g_t = f_t dh_t passing from row t to row t-1 (dh_t = dy_t + g_{t+1}), the same
+// holds with time reversed; h_{t-1} is recomputed from the state before every 16th row, which the
+// forward pass leaves behind (one row of floats for 16 rows of elements).
+//
+// Every element is read from and written to memory once.  Bound by HBM: 3 arrays forward, 5 backward.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -29,14 +28,19 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kRows       = 16;   // rows per warp and window
-constexpr int kWidth      = 64;   // channels per block
-constexpr int kChunk      = 64;   // spacing of the states
-constexpr int kChunkWarps = kChunk / kRows;
+constexpr int kLoneRows   = 32;  // rows per window of a warp that goes through a sequence alone
+constexpr int kJoinedRows = 16;  // and of one that shares it with others: more warps, each with less to do
+constexpr int kSpacing    = 16;  // of the states
+constexpr int kGroup      = 8;   // rows of the backward pass that are worked on side by side
+constexpr int kWidth      = 64;  // channels per warp
 constexpr int kMaxWarps   = 8;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxStages  = 6;    // windows in a warp's ring
-constexpr int kForwardBlocks = 2, kBackwardBlocks = 2;  // of 8 warps to an SM: 128 registers a thread
+constexpr int kMaxStages  = 3;   // windows in a warp's ring
+// Blocks of 8 warps that the registers of an SM hold.  The gradient of SIGMOID gates spills 400 bytes a thread at 128
+// registers, and is faster with half the warps (packed fp16, 37 sequences of 1000 channels: 165 us against 233).
+constexpr int kForwardBlocks = 2;
+template <int GATE>
+constexpr int kBackwardBlocks = GATE == TCU_GATE_SIGMOID ? 1 : 2;
 
 struct ScanArgs {
   const void *a, *x, *dh;
@@ -69,10 +73,16 @@ __device__ __forceinline__ void gate_of(float a, float& f, float& one_minus_f) {
   }
 }
 
-// The rows of the block's sequence: where they begin, how many, and where its chunks' states lie.
+template <int GATE>
+__device__ __forceinline__ void gate_of(float2 a, float2& f, float2& one_minus_f) {
+  gate_of<GATE>(a.x, f.x, one_minus_f.x);
+  gate_of<GATE>(a.y, f.y, one_minus_f.y);
+}
+
+// The rows of the block's sequence: where they begin, how many, and where its states lie.
 struct Sequence {
   int64_t a, x, dh, out;  // element offsets of the first row
-  int64_t chunk;          // row of `states` of the first chunk
+  int64_t chunk;          // row of `states` of the first rows
   int64_t length;
 };
 
@@ -84,7 +94,7 @@ __device__ __forceinline__ Sequence sequence_of(const ScanArgs& p, int64_t b) {
     s.x      = b * p.x_batch;
     s.dh     = b * p.dh_batch;
     s.out    = b * p.tokens * p.dim;
-    s.chunk  = b * ((p.tokens + kChunk - 1) / kChunk);
+    s.chunk  = b * ((p.tokens + kSpacing - 1) / kSpacing);
     return s;
   }
   int64_t first = load_index(p.offsets, b, p.wide), end = load_index(p.offsets, b + 1, p.wide);
@@ -97,7 +107,7 @@ __device__ __forceinline__ Sequence sequence_of(const ScanArgs& p, int64_t b) {
   s.x      = first * p.x_row;
   s.dh     = first * p.dh_row;
   s.out    = first * p.dim;
-  s.chunk  = first / kChunk + b;  // distinct: a sequence has at most length / kChunk + 1 chunks
+  s.chunk  = first / kSpacing + b;  // distinct: a sequence has at most length / kSpacing + 1 states
   return s;
 }
 
@@ -121,9 +131,9 @@ __device__ __forceinline__ void copy_wait(int pending) {
   }
 }
 
-// Copies rows row ... row + 15 (those that are below `length`) of the warp's channels, the first `left` of them,
+// Copies kRows rows from `row` on (those that are below `length`) of the warp's channels, the first `left` of them,
 // to `to`, kWidth elements a row.  `base`: the block's first channel in the sequence's first row.
-template <typename T>
+template <typename T, int kRows>
 __device__ __forceinline__ void copy_rows(T* to, const T* base, int64_t row_stride, int64_t row, int64_t length,
                                           int left, int piece) {
   const int lane = threadIdx.x & 31;
@@ -168,8 +178,9 @@ __device__ __forceinline__ void copy_rows(T* to, const T* base, int64_t row_stri
 // A lane's two channels of a row in shared memory.
 template <typename T>
 __device__ __forceinline__ float2 pair_at(const T* row) {
-  const Vec<T, 2> r = load_vec<T, 2>(row + (threadIdx.x & 31) * 2);
-  return make_float2(to_float(r.v[0]), to_float(r.v[1]));
+  float y[2];
+  to_floats<T, 2>(load_vec<T, 2>(row + (threadIdx.x & 31) * 2), y);
+  return make_float2(y[0], y[1]);
 }
 
 // Stores a lane's two channels, of which `count` exist.
@@ -183,17 +194,17 @@ __device__ __forceinline__ void store_pair(T* p, float2 x, int count, bool pairs
     if (count > 1) p[1] = from_float<T>(x.y);
   }
 }
-// Stores a lane's two channels of `rows` rows.
-template <typename T>
-__device__ __forceinline__ void store_rows(T* p, const float2 (&x)[kRows], int64_t dim, int rows, int count, bool pairs) {
-  if (rows == kRows && pairs) {
+// Stores a lane's two channels of N rows, `rows` of them if that is less.
+template <typename T, int N>
+__device__ __forceinline__ void store_rows(T* p, const float2 (&x)[N], int64_t dim, int rows, int count, bool pairs) {
+  if (rows >= N && pairs) {
     if (count > 0) {
 #pragma unroll
-      for (int i = 0; i < kRows; ++i, p += dim) store_pair<T>(p, x[i], 2, true);
+      for (int i = 0; i < N; ++i, p += dim) store_pair<T>(p, x[i], 2, true);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i, p += dim)
+    for (int i = 0; i < N; ++i, p += dim)
       if (i < rows) store_pair<T>(p, x[i], count, pairs);
   }
 }
@@ -229,20 +240,34 @@ struct Map {  // h -> a h + b, of a lane's two channels
   float2 a, b;
 };
 
+// What both kernels begin with: a block's place.
+struct Place {
+  int64_t b, first, ch;  // sequence, the block's first channel, the lane's
+  int left, count;       // channels of the block from `first`; of the lane: above 0, above 1
+};
+__device__ __forceinline__ Place place_of(const ScanArgs& p, int64_t group) {
+  Place w;
+  w.b     = group / p.columns;
+  w.first = group % p.columns * kWidth, w.ch = w.first + (threadIdx.x & 31) * 2;
+  w.left  = p.dim - w.first < kWidth ? int(p.dim - w.first) : kWidth;
+  w.count = w.left - int(threadIdx.x & 31) * 2;
+  return w;
+}
+
 // The maps of a block's warps and of a cluster's blocks, lanes side by side; two sets, used in turn.
 struct Maps {
   float2 warp_a[2][kMaxWarps][32], warp_b[2][kMaxWarps][32];
   float2 block_a[2][kMaxCluster][32], block_b[2][kMaxCluster][32];
 };
 
-// Joins the maps of all warps and blocks of the window: `state` goes from before the window to
-// behind it (REVERSE: time runs backwards, from the last block and warp to the first); returns the state this warp's rows
-// start from, and in `at_chunk` the one this warp's chunk starts from.
+// Joins the maps of all warps and blocks of a window: `state` goes from before them to behind them
+// (REVERSE: time runs backwards, from the last block and warp to the first); returns the state this warp's rows
+// start from.
 template <bool REVERSE>
-__device__ __forceinline__ float2 join_maps(Maps& m, const Map& mine, float2& state, float2& at_chunk, int side,
+__device__ __forceinline__ float2 join_maps(Maps& m, const Map& mine, float2& state, int side,
                                             const cg::cluster_group& cluster, int part, int parts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int at = REVERSE ? warps - 1 - warp : warp, chunk = at & ~(kChunkWarps - 1);
+  const int at = REVERSE ? warps - 1 - warp : warp;
   m.warp_a[side][at][lane] = finite(mine.a);
   m.warp_b[side][at][lane] = mine.b;
   __syncthreads();
@@ -256,11 +281,7 @@ __device__ __forceinline__ float2 join_maps(Maps& m, const Map& mine, float2& st
     }
     all.a = finite(all.a);
     const int place = REVERSE ? parts - 1 - part : part;
-    if (warp < parts) {
-      cluster.map_shared_rank(m.block_a[side][place], warp)[lane] = all.a;
-      cluster.map_shared_rank(m.block_b[side][place], warp)[lane] = all.b;
-    }
-    for (int q = warp + warps; q < parts; q += warps) {
+    for (int q = warp; q < parts; q += warps) {
       cluster.map_shared_rank(m.block_a[side][place], q)[lane] = all.a;
       cluster.map_shared_rank(m.block_b[side][place], q)[lane] = all.b;
     }
@@ -269,15 +290,9 @@ __device__ __forceinline__ float2 join_maps(Maps& m, const Map& mine, float2& st
       if (q == place) before = state;
       state = fma2(m.block_a[side][q][lane], state, m.block_b[side][q][lane]);
     }
-    at_chunk = before;
-    for (int j = 0; j < at; ++j) {
-      before = fma2(m.warp_a[side][j][lane], before, m.warp_b[side][j][lane]);
-      if (j + 1 == chunk) at_chunk = before;
-    }
+    for (int j = 0; j < at; ++j) before = fma2(m.warp_a[side][j][lane], before, m.warp_b[side][j][lane]);
   } else {
-    at_chunk = state;
     for (int j = 0; j < warps; ++j) {
-      if (j == chunk) at_chunk = state;
       if (j == at) before = state;
       state = fma2(m.warp_a[side][j][lane], state, m.warp_b[side][j][lane]);
     }
@@ -289,6 +304,7 @@ __device__ __forceinline__ float2 join_maps(Maps& m, const Map& mine, float2& st
 template <typename T, typename A, int GATE>
 __global__ void __launch_bounds__(kMaxWarps * 32, kForwardBlocks)
 linear_scan_kernel(const ScanArgs p) {
+  constexpr int kRows = kJoinedRows;
   __shared__ Maps maps;
   extern __shared__ __align__(16) unsigned char ring[];
   const cg::cluster_group cluster = cg::this_cluster();
@@ -314,8 +330,8 @@ linear_scan_kernel(const ScanArgs p) {
   auto fetch = [&](int64_t from, int stage) {
     A* to = reinterpret_cast<A*>(mine + stage * kStage);
     if (from < s.length) {
-      copy_rows<A>(to, a, p.a_row, from, s.length, left, p.a_piece);
-      copy_rows<T>(reinterpret_cast<T*>(to + kRows * kWidth), x, p.x_row, from, s.length, left, p.x_piece);
+      copy_rows<A, kRows>(to, a, p.a_row, from, s.length, left, p.a_piece);
+      copy_rows<T, kRows>(reinterpret_cast<T*>(to + kRows * kWidth), x, p.x_row, from, s.length, left, p.x_piece);
     }
     copy_commit();
   };
@@ -348,12 +364,11 @@ linear_scan_kernel(const ScanArgs p) {
       for (int i = 0; i < kRows; ++i)  // (rows behind the end: the identity)
         if (i < rows) map.b = fma2(f[i], map.b, input_at(i)), map.a = mul2(map.a, f[i]);
     }
-    float2 at_chunk;
-    float2 h = join_maps<false>(maps, map, state, at_chunk, side, cluster, part, parts);
-    if (p.states && warp % kChunkWarps == 0 && rows > 0) {
-      float* st = p.states + (s.chunk + row / kChunk) * p.dim + ch;
-      if (count > 0) st[0] = at_chunk.x;
-      if (count > 1) st[1] = at_chunk.y;
+    float2 h = join_maps<false>(maps, map, state, side, cluster, part, parts);
+    if (p.states && rows > 0) {
+      float* st = p.states + (s.chunk + row / kSpacing) * p.dim + ch;
+      if (count > 0) st[0] = h.x;
+      if (count > 1) st[1] = h.y;
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) f[i] = h = fma2(f[i], h, input_at(i));
@@ -371,30 +386,27 @@ linear_scan_kernel(const ScanArgs p) {
 }
 
 // ------------------------------------------------------------------ backward
-template <typename T, typename A, int GATE>
-__global__ void __launch_bounds__(kMaxWarps * 32, kBackwardBlocks)
+// JOINED: the warps of a block and the blocks of a cluster share a sequence's time; else a block is one warp.
+template <typename T, typename A, int GATE, bool JOINED>
+__global__ void __launch_bounds__(JOINED ? kMaxWarps * 32 : 32, JOINED ? kBackwardBlocks<GATE> : 1)
 linear_scan_backward_kernel(const ScanArgs p) {
-  __shared__ Maps maps;
-  __shared__ float2 forward_a[2][kMaxWarps][32], forward_b[2][kMaxWarps][32];
+  constexpr int kRows = JOINED ? kJoinedRows : kLoneRows;
+  __shared__ typename std::conditional<JOINED, Maps, int>::type maps;
   extern __shared__ __align__(16) unsigned char ring[];
   const cg::cluster_group cluster = cg::this_cluster();
-  const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int64_t group = blockIdx.x / parts;
-  const int64_t b     = group / p.columns;
-  const int64_t first = (group % p.columns) * kWidth, ch = first + lane * 2;
-  const int left = p.dim - first < kWidth ? int(p.dim - first) : kWidth;
-  const int count = left - lane * 2;
-  const Sequence s = sequence_of(p, b);
-  const A* a  = static_cast<const A*>(p.a) + s.a + first;
-  const T* x  = static_cast<const T*>(p.x) + s.x + first;
-  const T* dy = static_cast<const T*>(p.dh) + s.dh + first;
-  A* da       = static_cast<A*>(p.da) + s.out + ch;
-  T* dx       = static_cast<T*>(p.dx) + s.out + ch;
+  const int parts = JOINED ? int(cluster.num_blocks()) : 1, part = JOINED ? int(cluster.block_rank()) : 0;
+  const int warp = JOINED ? threadIdx.x >> 5 : 0, warps = JOINED ? blockDim.x >> 5 : 1;
+  const Place w    = place_of(p, blockIdx.x / parts);
+  const Sequence s = sequence_of(p, w.b);
+  const A* a  = static_cast<const A*>(p.a) + s.a + w.first;
+  const T* x  = static_cast<const T*>(p.x) + s.x + w.first;
+  const T* dy = static_cast<const T*>(p.dh) + s.dh + w.first;
+  A* da       = static_cast<A*>(p.da) + s.out + w.ch;
+  T* dx       = static_cast<T*>(p.dx) + s.out + w.ch;
   const bool has_dy = p.dh != nullptr;
-
-  float2 state = p.dlast ? load_pair(p.dlast + b * p.dim + ch, count) : make_float2(0.f, 0.f);  // passed back by the rows behind
-  if (parts > 1) cluster.sync();
+  // what the rows behind the window pass back
+  float2 state = p.dlast ? load_pair(p.dlast + w.b * p.dim + w.ch, w.count) : make_float2(0.f, 0.f);
+  if (parts > 1) cluster.sync();  // no block writes to another's shared memory before that has begun
 
   constexpr int kStage  = kRows * kWidth * int(sizeof(A) + 2 * sizeof(T));
   unsigned char* mine   = ring + warp * p.stages * kStage;
@@ -405,99 +417,113 @@ linear_scan_backward_kernel(const ScanArgs p) {
     A* to = reinterpret_cast<A*>(mine + stage * kStage);
     T* tx = reinterpret_cast<T*>(to + kRows * kWidth);
     if (from >= 0 && from < s.length) {
-      copy_rows<A>(to, a, p.a_row, from, s.length, left, p.a_piece);
-      copy_rows<T>(tx, x, p.x_row, from, s.length, left, p.x_piece);
-      if (has_dy) copy_rows<T>(tx + kRows * kWidth, dy, p.dh_row, from, s.length, left, p.dh_piece);
+      copy_rows<A, kRows>(to, a, p.a_row, from, s.length, w.left, p.a_piece);
+      copy_rows<T, kRows>(tx, x, p.x_row, from, s.length, w.left, p.x_piece);
+      if (has_dy) copy_rows<T, kRows>(tx + kRows * kWidth, dy, p.dh_row, from, s.length, w.left, p.dh_piece);
     }
     copy_commit();
   };
+  auto state_at = [&](int64_t from) {  // the state before row `from` of the sequence
+    return from >= 0 && from < s.length ? load_pair(p.states + (s.chunk + from / kSpacing) * p.dim + w.ch, w.count)
+                                        : make_float2(0.f, 0.f);
+  };
   for (int i = 0; i < p.stages; ++i) fetch(row - i * step, i);
-  int side = 0, stage = 0;
-  for (int64_t window = 0; window < windows; ++window, row -= step, side ^= 1) {
+  int stage = 0;
+  constexpr int kParts = kRows / kSpacing;
+  float2 next_h[kParts];
+#pragma unroll
+  for (int k = 0; k < kParts; ++k) next_h[k] = state_at(row + k * kSpacing);
+  for (uint32_t n = 0; n < windows; ++n, row -= step) {
     const int rows = s.length - row < kRows ? int(s.length - row) : kRows;
-    float2 h = make_float2(0.f, 0.f);  // the state before this warp's chunk of rows
-    if (rows > 0) h = load_pair(p.states + (s.chunk + row / kChunk) * p.dim + ch, count);
+    float2 h[kParts];
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) h[k] = next_h[k], next_h[k] = state_at(row - step + k * kSpacing);
     copy_wait(p.stages - 1);
     __syncwarp();
     const A* sa = reinterpret_cast<const A*>(mine + stage * kStage);
     const T* sx = reinterpret_cast<const T*>(sa + kRows * kWidth);
     const T* sd = sx + kRows * kWidth;
-    float2 f[kRows], rest[kRows];  // rest: 1 - f, SIGMOID only
-    Map forward = {make_float2(1.f, 1.f), make_float2(0.f, 0.f)}, back = forward;
-    auto gradient_at = [&](int i) {  // dy of row i
-      return has_dy ? pair_at<T>(sd + i * kWidth) : make_float2(0.f, 0.f);
+    // gates of rows i ... i + kGroup - 1
+    auto gates_at = [&](int i, float2 (&f)[kGroup], float2 (&rest)[kGroup]) {
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) f[k] = pair_at<A>(sa + (i + k) * kWidth);
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) gate_of<GATE>(f[k], f[k], rest[k]);
     };
-    auto input_at = [&](int i) {  // u of row i
-      const float2 gx = pair_at<T>(sx + i * kWidth);
-      if constexpr (GATE == TCU_GATE_SIGMOID) return mul2(rest[i], gx);
-      return gx;
-    };
+    // dy of rows i ... i + kGroup - 1; the rows from `rows` on pass on what they get: f 1 and dy 0
+    auto gradients_at = [&](int i, float2 (&d)[kGroup], float2 (&f)[kGroup]) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const float2 ga = pair_at<A>(sa + i * kWidth);
-      gate_of<GATE>(ga.x, f[i].x, rest[i].x);
-      gate_of<GATE>(ga.y, f[i].y, rest[i].y);
-    }
-    auto first_pass = [&](auto whole) {
-      constexpr bool kWhole = decltype(whole)::value;
+      for (int k = 0; k < kGroup; ++k) d[k] = has_dy ? pair_at<T>(sd + (i + k) * kWidth) : make_float2(0.f, 0.f);
+      if (i + kGroup > rows) {
 #pragma unroll
-      for (int i = 0; i < kRows; ++i)
-        if (kWhole || i < rows) forward.b = fma2(f[i], forward.b, input_at(i)), forward.a = mul2(forward.a, f[i]);
-#pragma unroll
-      for (int i = kRows - 1; i >= 0; --i)
-        if (kWhole || i < rows) back.b = mul2(f[i], add2(gradient_at(i), back.b));
-    };
-    if (rows == kRows)
-      first_pass(std::true_type{});
-    else
-      first_pass(std::false_type{});
-    back.a = forward.a;
-    forward_a[side][warp][lane] = finite(forward.a);
-    forward_b[side][warp][lane] = forward.b;
-    float2 unused;
-    float2 g = join_maps<true>(maps, back, state, unused, side, cluster, part, parts);
-    for (int j = warp & ~(kChunkWarps - 1); j < warp; ++j) h = fma2(forward_a[side][j][lane], h, forward_b[side][j][lane]);
-    float2 before[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      before[i] = h;
-      h         = fma2(f[i], h, input_at(i));
-    }
-    // before becomes da, f becomes dx
-    auto second_pass = [&](auto whole) {
-#pragma unroll
-      for (int i = kRows - 1; i >= 0; --i) {
-        if (!decltype(whole)::value && i >= rows) continue;
-        const float2 dh = add2(gradient_at(i), g), fi = f[i];
-        g = mul2(fi, dh);
-        if constexpr (GATE == TCU_GATE_SIGMOID) {
-          const float2 v = pair_at<T>(sx + i * kWidth);
-          before[i] = mul2(mul2(dh, add2(before[i], make_float2(-v.x, -v.y))), mul2(fi, rest[i]));
-          f[i]      = mul2(dh, rest[i]);
-        } else {
-          before[i] = mul2(GATE == TCU_GATE_LOG ? g : dh, before[i]);
-          f[i]      = dh;
-        }
+        for (int k = 0; k < kGroup; ++k)
+          if (i + k >= rows) f[k] = make_float2(1.f, 1.f), d[k] = make_float2(0.f, 0.f);
       }
     };
-    if (rows == kRows)
-      second_pass(std::true_type{});
-    else
-      second_pass(std::false_type{});
-    store_rows<A>(da + row * p.dim, before, p.dim, rows, count, p.pairs);
-    store_rows<T>(dx + row * p.dim, f, p.dim, rows, count, p.pairs);
+    float2 g = state;
+    if constexpr (JOINED) {
+      // g passes back f_0 (dy_0 + f_1 (dy_1 + ...)), the sum of dy_i times the product of f_0 ... f_i
+      Map back = {make_float2(1.f, 1.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+      for (int i = 0; i < kRows; i += kGroup) {
+        float2 f[kGroup], rest[kGroup], d[kGroup];
+        gates_at(i, f, rest);
+        gradients_at(i, d, f);
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) back.a = mul2(back.a, f[k]), back.b = fma2(back.a, d[k], back.b);
+      }
+      g = join_maps<true>(maps, back, state, n & 1, cluster, part, parts);
+    }
+    float2 before[kRows];
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+      for (int i = part * kSpacing; i < (part + 1) * kSpacing; i += kGroup) {
+        float2 f[kGroup], rest[kGroup], u[kGroup];
+        gates_at(i, f, rest);
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) {
+          u[k] = pair_at<T>(sx + (i + k) * kWidth);
+          if constexpr (GATE == TCU_GATE_SIGMOID) u[k] = mul2(rest[k], u[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) before[i + k] = h[part], h[part] = fma2(f[k], h[part], u[k]);
+      }
+    }
+#pragma unroll
+    for (int i = kRows - kGroup; i >= 0; i -= kGroup) {
+      if (i >= rows) continue;
+      float2 f[kGroup], rest[kGroup], d[kGroup], ga[kGroup];
+      gates_at(i, f, rest);
+      gradients_at(i, d, f);
+#pragma unroll
+      for (int k = kGroup - 1; k >= 0; --k) {
+        d[k] = add2(d[k], g);  // dh
+        g    = mul2(f[k], d[k]);
+        if constexpr (GATE == TCU_GATE_SIGMOID) {
+          const float2 v = pair_at<T>(sx + (i + k) * kWidth);
+          ga[k] = mul2(mul2(d[k], add2(before[i + k], make_float2(-v.x, -v.y))), mul2(f[k], rest[k]));
+          d[k]  = mul2(d[k], rest[k]);
+        } else {
+          ga[k] = mul2(GATE == TCU_GATE_LOG ? g : d[k], before[i + k]);
+        }
+      }
+      store_rows<A>(da + (row + i) * p.dim, ga, p.dim, rows - i, w.count, p.pairs);
+      store_rows<T>(dx + (row + i) * p.dim, d, p.dim, rows - i, w.count, p.pairs);
+    }
+    if constexpr (!JOINED) state = g;
     __syncwarp();
     fetch(row - p.stages * step, stage);
     stage = stage + 1 == p.stages ? 0 : stage + 1;
   }
   if (p.clear_rest) {
-    clear_rest<A>(p, static_cast<A*>(p.da) + ch, b, count, part, parts);
-    clear_rest<T>(p, static_cast<T*>(p.dx) + ch, b, count, part, parts);
+    clear_rest<A>(p, static_cast<A*>(p.da) + w.ch, w.b, w.count, part, parts);
+    clear_rest<T>(p, static_cast<T*>(p.dx) + w.ch, w.b, w.count, part, parts);
   }
   if (p.dh0 && part == 0 && warp == 0) {
-    float* dh0 = p.dh0 + b * p.dim + ch;
-    if (count > 0) dh0[0] = state.x;
-    if (count > 1) dh0[1] = state.y;
+    float* dh0 = p.dh0 + w.b * p.dim + w.ch;
+    if (w.count > 0) dh0[0] = state.x;
+    if (w.count > 1) dh0[1] = state.y;
   }
 }
 
@@ -587,39 +613,54 @@ int piece_of(const void* p, size_t elem, int64_t dim, int64_t batch_stride, int6
   return fits(16) ? 16 : fits(4) ? 4 : int(elem);
 }
 
-constexpr int kSharedPerSm = 220 << 10;
+constexpr int kSharedPerSm = 224 << 10;
 
-// Warps per block and blocks per cluster: as many as it takes to give every SM kWarpsWanted warps, if the
-// sequences have the rows for them; blocks of 8 warps before clusters, which have to meet.  Stages: what then fits.
-constexpr int kWarpsWanted = 8;
+// With eight columns of 64 channels for every SM a warp goes through a sequence alone.  With fewer, time is
+// cut: blocks of 8 warps (fewer where their rings would not leave room for a second block on the SM, or all blocks would
+// not fit on the SMs at once), and with fewer columns than SMs clusters of up to 8 such blocks, as
+// long as the sequences have the rows for them.  (Clusters of 8 blocks that fill an SM each do not all find 8 free SMs
+// side by side: 15 of 16 did.)  A ring takes what shared memory is left, two windows at least.
+constexpr int kLoneColumns = 8;
 
-template <void (*Kernel)(const ScanArgs)>
-cudaError_t launch_clusters(ScanArgs args, int stage_bytes, int static_bytes, int sms, cudaStream_t st) {
-  args.columns         = int((args.dim + kWidth - 1) / kWidth);
-  const int64_t groups = args.batch * args.columns;
-  const int64_t each   = args.offsets ? 2 * args.tokens / args.batch : args.tokens;
-  int warps = kChunkWarps, parts = 1;
-  auto more = [&] { return groups * parts * warps < int64_t(sms) * kWarpsWanted && each > int64_t(parts) * warps * kRows; };
-  if (more()) warps = kMaxWarps;
-  while (parts < kMaxCluster && more()) parts *= 2;
-  if (groups * parts > int64_t(0x7fffffff)) return cudaErrorInvalidConfiguration;
-  const int64_t per_sm = (groups * parts + sms - 1) / sms;  // blocks that there are for an SM
-  int stages = 2;
-  while (stages < kMaxStages && per_sm * ((stages + 1) * warps * stage_bytes + static_bytes) <= kSharedPerSm) ++stages;
-  args.stages     = stages;
-  const int bytes = stages * warps * stage_bytes;
+template <void (*Lone)(const ScanArgs), void (*Joined)(const ScanArgs)>
+cudaError_t launch_scan(ScanArgs args, int row_bytes, int blocks, int sms, cudaStream_t st) {
+  constexpr int kStatic = int(sizeof(Maps));  // of a joined block
   static bool configured[kMaxDevices];
   const int dev = current_device();
   if (dev < 0) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedPerSm - static_bytes);
+    cudaError_t e = cudaFuncSetAttribute(Lone, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedPerSm - kStatic);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(Joined, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedPerSm - kStatic);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
+  args.columns         = int((args.dim + kWidth - 1) / kWidth);
+  const int64_t groups = args.batch * args.columns;
+  const int64_t each   = args.offsets ? 2 * args.tokens / args.batch : args.tokens;  // (packed: a guess)
+  int warps = 1, parts = 1;
+  auto bytes_of = [&](int stages) {
+    return stages * warps * row_bytes * (warps > 1 ? kJoinedRows : kLoneRows);
+  };
+  auto fit = [&] {  // blocks on an SM
+    const int by_memory = kSharedPerSm / (bytes_of(2) + kStatic + 1024), by_registers = blocks * kMaxWarps / warps;
+    return by_memory < by_registers ? by_memory : by_registers;
+  };
+  if (Lone == Joined || (groups < int64_t(kLoneColumns) * sms && each > kLoneRows)) {
+    warps = kMaxWarps;
+    while (warps > 2 && (2 * (bytes_of(2) + 17 * 1024) > (226 << 10) || (warps > 4 && groups > int64_t(sms) * fit())))
+      warps /= 2;
+    while (parts < kMaxCluster && groups * parts < sms && each > int64_t(parts) * warps * kJoinedRows) parts *= 2;
+  }
+  if (groups * parts > int64_t(0x7fffffff)) return cudaErrorInvalidConfiguration;
+  int64_t per_sm = (groups * parts + sms - 1) / sms;  // blocks that there are for an SM
+  int stages = 2;
+  while (parts == 1 && stages < kMaxStages && per_sm * (bytes_of(stages + 1) + (warps > 1 ? kStatic : 0) + 1024) <= kSharedPerSm) ++stages;
+  args.stages            = stages;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim            = dim3(unsigned(groups * parts));
   cfg.blockDim           = dim3(warps * 32);
-  cfg.dynamicSmemBytes   = bytes;
+  cfg.dynamicSmemBytes   = bytes_of(stages);
   cfg.stream             = st;
   cudaLaunchAttribute attr[1];
   attr[0].id                 = cudaLaunchAttributeClusterDimension;
@@ -628,7 +669,7 @@ cudaError_t launch_clusters(ScanArgs args, int stage_bytes, int static_bytes, in
   attr[0].val.clusterDim.z   = 1;
   cfg.attrs    = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, Kernel, args);
+  return cudaLaunchKernelEx(&cfg, warps > 1 ? Joined : Lone, args);
 }
 
 bool bad_sizes(int64_t batch, int64_t tokens, int64_t dim) {
@@ -645,7 +686,7 @@ using namespace tcu_lm;
 extern "C" {
 
 size_t tcu_linear_scan_states_rows(size_t batch, size_t tokens, int packed) {
-  return packed ? tokens / kChunk + batch : batch * ((tokens + kChunk - 1) / kChunk);
+  return packed ? tokens / kSpacing + batch : batch * ((tokens + kSpacing - 1) / kSpacing);
 }
 
 int tcu_linear_scan(const tcu_linear_scan_args* g, void* stream) {
@@ -672,9 +713,9 @@ int tcu_linear_scan(const tcu_linear_scan_args* g, void* stream) {
   const cudaError_t err = for_types(g->type, g->a_type, g->gate, [&](auto t, auto a, auto gate) {
     using T = decltype(t);
     using A = decltype(a);
-    return launch_clusters<linear_scan_kernel<T, A, decltype(gate)::value>>(
-        p, kRows * kWidth * int(sizeof(A) + sizeof(T)),
-                           sizeof(Maps), sms, static_cast<cudaStream_t>(stream));
+    constexpr int G = decltype(gate)::value;
+    return launch_scan<linear_scan_kernel<T, A, G>, linear_scan_kernel<T, A, G>>(
+        p, kWidth * int(sizeof(A) + sizeof(T)), kForwardBlocks, sms, static_cast<cudaStream_t>(stream));
   });
   return err == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
 }
@@ -707,9 +748,9 @@ int tcu_linear_scan_backward(const tcu_linear_scan_backward_args* g, void* strea
   const cudaError_t err = for_types(g->type, g->a_type, g->gate, [&](auto t, auto a, auto gate) {
     using T = decltype(t);
     using A = decltype(a);
-    return launch_clusters<linear_scan_backward_kernel<T, A, decltype(gate)::value>>(
-        p, kRows * kWidth * int(sizeof(A) + 2 * sizeof(T)), sizeof(Maps) + 4 * kMaxWarps * 32 * 8, sms,
-                           static_cast<cudaStream_t>(stream));
+    constexpr int G = decltype(gate)::value;
+    return launch_scan<linear_scan_backward_kernel<T, A, G, false>, linear_scan_backward_kernel<T, A, G, true>>(
+        p, kWidth * int(sizeof(A) + 2 * sizeof(T)), kBackwardBlocks<G>, sms, static_cast<cudaStream_t>(stream));
   });
   return err == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
 }

@@ -10,6 +10,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace tcu_lm {
 
 constexpr int kMaxDevices = 64;
@@ -22,6 +24,9 @@ constexpr unsigned kErrIndex = 8u;
 static __device__ unsigned int g_lm_error_word;
 
 __device__ __forceinline__ void raise_index_error() { atomicOr(&g_lm_error_word, kErrIndex); }
+
+// Bit 0, as in the other kernels: an mbarrier wait ran out.
+constexpr unsigned kErrBarrier = 1u;
 
 // ------------------------------------------------------------------ elements
 // (16 bytes are the widest access: longer vectors are several of them)
@@ -54,12 +59,52 @@ __device__ __forceinline__ Vec<T, V> zero_vec() {
   for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(0.f);
   return r;
 }
+// Two elements to and from floats: one instruction to round and pack them, one each to unpack.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t x) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+
+// V elements, converted.
+template <typename T, int V>
+__device__ __forceinline__ void to_floats(const Vec<T, V>& x, float (&y)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 f = unpack_pair<T>(w[i]);
+      y[2 * i] = f.x, y[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = to_float(x.v[i]);
+  }
+}
+
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
-  Vec<T, V> r;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    Vec<uint32_t, V / 2> r;
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(x[i]);
-  *reinterpret_cast<Vec<T, V>*>(p) = r;
+    for (int i = 0; i < V / 2; ++i) r.v[i] = pack_pair<T>(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<Vec<uint32_t, V / 2>*>(p) = r;
+  } else {
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(x[i]);
+    *reinterpret_cast<Vec<T, V>*>(p) = r;
+  }
 }
 
 // An index array of 32 or 64 bits.

@@ -71,8 +71,10 @@ __device__ __forceinline__ void load_part(float (&x)[E], const void* row, int64_
   for (int k = 0; k < E / VEC; ++k) {
     const int at = (first + k * width) * VEC;
     const Vec<T, VEC> r = at < dim ? load_vec<T, VEC>(p + at) : zero_vec<T, VEC>();
+    float y[VEC];
+    to_floats<T, VEC>(r, y);
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) x[k * VEC + c] = to_float(r.v[c]);
+    for (int c = 0; c < VEC; ++c) x[k * VEC + c] = y[c];
   }
 }
 

@@ -95,9 +95,7 @@ struct Block16 {
   __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
   __device__ __forceinline__ float2 pair(int i) const {
     if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
-    const uint32_t x = word(i);
-    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&x));
-    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    else return unpack_pair<T>(word(i));
   }
   __device__ __forceinline__ float element(int c) const {
     const float2 x = pair(c / 2);

@@ -114,7 +114,7 @@ def _strides(t: torch.Tensor | None):
 
 
 def linear_scan_states(x: torch.Tensor, offsets: torch.Tensor | None = None) -> torch.Tensor:
-    """An uninitialised tensor for the ``states`` of :func:`linear_scan`: one row of floats for every 64 tokens."""
+    """An uninitialised tensor for the ``states`` of :func:`linear_scan`: one row of floats for every 16 tokens."""
     if offsets is None:
         rows = _lib.load().tcu_linear_scan_states_rows(x.size(0), x.size(1), 0)
     else:

@@ -79,8 +79,8 @@ def test_null_arguments(lib):
 
 
 def test_states_rows(lib):
-    assert lib.tcu_linear_scan_states_rows(3, 64, 0) == 3 and lib.tcu_linear_scan_states_rows(3, 65, 0) == 6
-    assert lib.tcu_linear_scan_states_rows(3, 65, 1) == 4 and lib.tcu_linear_scan_states_rows(3, 0, 0) == 0
+    assert lib.tcu_linear_scan_states_rows(3, 16, 0) == 3 and lib.tcu_linear_scan_states_rows(3, 17, 0) == 6
+    assert lib.tcu_linear_scan_states_rows(3, 17, 1) == 4 and lib.tcu_linear_scan_states_rows(3, 0, 0) == 0
 
 
 def test_python_structs_match_the_header(built_library):
