@@ -112,25 +112,6 @@ __device__ __forceinline__ Sequence sequence_of(const ScanArgs& p, int64_t b) {
 }
 
 // ------------------------------------------------------------------ the ring
-__device__ __forceinline__ void copy_async16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_async4(void* to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Returns when all but the newest `pending` groups of this thread have arrived.
-__device__ __forceinline__ void copy_wait(int pending) {
-  switch (pending) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-  }
-}
-
 // Copies kRows rows from `row` on (those that are below `length`) of the warp's channels, the first `left` of them,
 // to `to`, kWidth elements a row.  `base`: the block's first channel in the sequence's first row.
 template <typename T, int kRows>

@@ -2,18 +2,24 @@
 //     n = z / rms(z) * post        (z itself without post)
 //     o = residual + scale * act(gate) * n
 //     u = o / rms(o) * pre         rms(y) = sqrt(mean(y^2) + eps)
-// Row sums of squares of two arrays, the second known only after the first sum: a row stays in the
-// registers of one block (or warp) between its single read and its single write.
+// With c = scale act(gate) post, which rows share, and a = 1 / rms(z), o = residual + a c z, so that the second
+// norm's sum is known from sums that need no first:
+//     sum o^2 = sum residual^2 + 2 a sum residual c z + a^2 sum (c z)^2
+// and threads meet once a row.  Where the branch cancels most of the residual (sum o^2 below a quarter of what is
+// added up) that would lose digits, and o is summed itself, at another meeting.
 //
-// Gradient, per row, with v = du pre, on = o / rms(o), zn = z / rms(z):
-//     d  = do + (v - on mean(v on)) / rms(o)     = dresidual
-//     dn = scale act(gate) d,   w = dn post
-//     dz = (w - zn mean(w zn)) / rms(z)
-//     dpre = sum over rows of du on, dpost = sum of dn zn, dgate = sum of scale act'(gate) d n
+// Gradient, per row, with v = du pre, b = 1 / rms(o), zn = a z:
+//     d  = do + b (v - o b mean(v o b))                 = dresidual
+//     dz = a (c d - zn mean(c d zn))
+//     dpre = sum over rows of du o b;  q = sum over rows of d zn;  dpost = scale act(gate) q;  dgate = scale act'(gate) post q
+// and again every mean follows from sums of products of what is read:
+//     sum v o = sum v residual + a sum v c z
+//     sum c d z = sum c z do + b sum v c z - b^2 mean(v o b) (sum residual c z + a sum (c z)^2)
 // The sums over rows are kept by every block for its own rows, in registers, and joined by a second kernel in
 // the order of the blocks: no atomics, the same bits every time.
 //
-// Bound by HBM: 4 arrays forward, 6 backward.
+// Bound by HBM: 4 arrays forward, 6 backward.  Rows come through a ring in shared memory, each thread copying (cp.async)
+// what it will read itself: nothing is waited for but a thread's own copies and the one meeting.
 #include <type_traits>
 
 #include "lm_common.cuh"
@@ -27,50 +33,77 @@ struct NormArgs {
   const void *z, *residual, *post, *gate, *pre, *dout, *dnormed;
   void *out, *normed, *dz, *dresidual;
   void* dgate;        // written where one worker holds all rows of a gate row
-  float* gate_parts;  // else one row of floats per worker
+  float* gate_parts;  // else one row of floats per unit
   float *post_parts, *pre_parts;  // one row of floats per worker
   int64_t rows, rows_per_gate, slice_rows;
   int64_t z_row, residual_row, gate_row, dout_row, dnormed_row;
   int64_t units;      // backward: slices of the rows of one gate row
-  int64_t workers;    // blocks, or warps, that take consecutive units
+  int64_t workers;    // blocks, or warps, that take consecutive units (forward: rows)
   int slices;         // per gate row
-  int dim, act;
+  int dim, act, row_bytes;  // row_bytes: of a row in the ring
   float scale, eps;
 };
 
 __device__ __forceinline__ float act_of(int act, float g) {
   if (act == kNone) return g;
-  const float s = __fdividef(1.f, 1.f + expf(-g));
+  const float s = reciprocal(1.f + exp2_fast(-g * kLog2E));
   return act == kSigmoid ? s : g * s;
 }
 
 __device__ __forceinline__ float slope_of(int act, float g) {
   if (act == kNone) return 1.f;
-  const float s = __fdividef(1.f, 1.f + expf(-g)), r = __fdividef(1.f, 1.f + expf(g));  // r = 1 - s
+  const float s = reciprocal(1.f + exp2_fast(-g * kLog2E)), r = reciprocal(1.f + exp2_fast(g * kLog2E));  // r = 1 - s
   return act == kSigmoid ? s * r : s * (1.f + g * r);
 }
 
-// Sum over the threads of a row: a warp (WARP) or the block.  `scratch`: 32 floats that the previous
-// call did not use.  Every thread gets the sum, always added up in the same order.
-template <bool WARP>
-__device__ __forceinline__ float row_sum(float x, float* scratch) {
-  x = warp_sum(x);
-  if constexpr (WARP) return x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  if (warps == 1) return x;
-  if (lane == 0) scratch[warp] = x;
-  __syncthreads();
-  return warp_sum(lane < warps ? scratch[lane] : 0.f);
+// ------------------------------------------------------------------ sums over a row's threads
+// Each of N sums over a warp (WARP) or the block, in every thread, always added up in the same order: the
+// lanes halve the sums among them, so that 8 take 9 exchanges and not 40.  `scratch`: N x 33 floats that the previous
+// call did not use.
+template <bool WARP, int N>
+__device__ __forceinline__ void row_sums(float (&s)[N], float* scratch) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kLanes = 32 / N;  // lanes that end up with the same sum
+  int o = 16;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n /= 2, o /= 2) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = lane & o ? s[i + n] : s[i], give = lane & o ? s[i] : s[i + n];
+      s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  float x = s[0];
+#pragma unroll
+  for (int q = kLanes / 2; q >= 1; q /= 2) x += __shfl_xor_sync(0xffffffffu, x, q);
+  if constexpr (!WARP) {
+    const int warps = blockDim.x >> 5, mine = lane / kLanes, sub = lane % kLanes;
+    if (warps > 1) {
+      if (sub == 0) scratch[mine * 33 + (threadIdx.x >> 5)] = x;
+      __syncthreads();
+      x = 0.f;
+      for (int w = sub; w < warps; w += kLanes) x += scratch[mine * 33 + w];
+#pragma unroll
+      for (int q = kLanes / 2; q >= 1; q /= 2) x += __shfl_xor_sync(0xffffffffu, x, q);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = __shfl_sync(0xffffffffu, x, i * kLanes);
 }
 
-// Elements v * VEC ... of a row that this thread holds, v = first, first + width, ...: E in all.
+// ------------------------------------------------------------------ rows
+// A thread's elements of a row: vectors first, first + width, ... of VEC elements, E elements in all.
+template <int VEC, int E>
+struct Part {
+  int first, width, dim;
+  __device__ __forceinline__ int at(int k) const { return (first + k * width) * VEC; }
+};
+
 template <typename T, int VEC, int E>
-__device__ __forceinline__ void load_part(float (&x)[E], const void* row, int64_t offset, int first, int width, int dim) {
-  const T* p = static_cast<const T*>(row) + offset;
+__device__ __forceinline__ void load_part(float (&x)[E], const Part<VEC, E>& t, const T* row) {
 #pragma unroll
   for (int k = 0; k < E / VEC; ++k) {
-    const int at = (first + k * width) * VEC;
-    const Vec<T, VEC> r = at < dim ? load_vec<T, VEC>(p + at) : zero_vec<T, VEC>();
+    const Vec<T, VEC> r = t.at(k) < t.dim ? load_vec<T, VEC>(row + t.at(k)) : zero_vec<T, VEC>();
     float y[VEC];
     to_floats<T, VEC>(r, y);
 #pragma unroll
@@ -79,164 +112,263 @@ __device__ __forceinline__ void load_part(float (&x)[E], const void* row, int64_
 }
 
 template <typename T, int VEC, int E>
-__device__ __forceinline__ void store_part(void* row, int64_t offset, const float (&x)[E], int first, int width, int dim) {
-  T* p = static_cast<T*>(row) + offset;
+__device__ __forceinline__ void store_part(T* row, const Part<VEC, E>& t, const float (&x)[E]) {
 #pragma unroll
   for (int k = 0; k < E / VEC; ++k) {
-    const int at = (first + k * width) * VEC;
     float y[VEC];
 #pragma unroll
     for (int c = 0; c < VEC; ++c) y[c] = x[k * VEC + c];
-    if (at < dim) store_vec<T, VEC>(p + at, y);
+    if (t.at(k) < t.dim) store_vec<T, VEC>(row + t.at(k), y);
   }
 }
 
-template <typename T, typename W, int VEC, int E, bool WARP, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+constexpr int kStages = 3;  // rows in the ring
+
+// An array's rows on their way through the ring (VEC == 1: read from where they are; those rows are not
+// aligned for copies).
+template <typename T, int VEC, int E>
+struct Stream {
+  const T* base;
+  int64_t stride;
+  unsigned char* ring;  // of stage 0
+  int stage_bytes;
+
+  __device__ __forceinline__ void fetch(const Part<VEC, E>& t, int64_t row, int stage) const {
+    if (VEC == 1 || base == nullptr) return;
+    const T* from = base + row * stride;
+    T* to         = reinterpret_cast<T*>(ring + stage * stage_bytes);
+#pragma unroll
+    for (int k = 0; k < E / VEC; ++k)
+      if (t.at(k) < t.dim) copy_async16(to + t.at(k), from + t.at(k));
+  }
+  __device__ __forceinline__ void load(float (&x)[E], const Part<VEC, E>& t, int64_t row, int stage) const {
+    if (base == nullptr) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = 0.f;
+    } else {
+      load_part<T, VEC, E>(x, t, VEC == 1 ? base + row * stride : reinterpret_cast<const T*>(ring + stage * stage_bytes));
+    }
+  }
+};
+
+// c = scale act(gate) post, of the gate's row `group`.
+template <typename T, typename W, int VEC, int E>
+__device__ __forceinline__ void coefficients(float (&c)[E], const Part<VEC, E>& t, const NormArgs& p, int64_t group) {
+#pragma unroll
+  for (int i = 0; i < E; ++i) c[i] = p.scale;
+  float x[E];
+  if (p.gate) {
+    load_part<T, VEC, E>(x, t, static_cast<const T*>(p.gate) + group * p.gate_row);
+#pragma unroll
+    for (int i = 0; i < E; ++i) c[i] *= act_of(p.act, x[i]);
+  }
+  if (p.post) {
+    load_part<W, VEC, E>(x, t, static_cast<const W*>(p.post));
+#pragma unroll
+    for (int i = 0; i < E; ++i) c[i] *= x[i];
+  }
+}
+
+// Whether sum o^2, of terms of this size, has lost digits.
+__device__ __forceinline__ bool cancelled(float sum, float residual_part, float branch_part) {
+  return sum < 0.25f * (residual_part + branch_part);
+}
+
+template <typename T, typename W, int VEC, int E, bool WARP, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS)
 norm_residual_kernel(const NormArgs p) {
-  __shared__ float scratch[2][32];
-  const int first = WARP ? threadIdx.x & 31 : threadIdx.x, width = WARP ? 32 : blockDim.x;
-  const int64_t workers = WARP ? int64_t(gridDim.x) * (THREADS / 32) : gridDim.x;
-  int64_t row           = WARP ? int64_t(blockIdx.x) * (THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
-  const float inv_dim   = 1.f / float(p.dim);
-  for (; row < p.rows; row += workers) {
-    float z[E], o[E];
-    load_part<T, VEC, E>(z, p.z, row * p.z_row, first, width, p.dim);
-    if (p.residual)
-      load_part<T, VEC, E>(o, p.residual, row * p.residual_row, first, width, p.dim);
-    else {
+  __shared__ float scratch[2][4 * 33], again[2][2 * 33];
+  extern __shared__ __align__(16) unsigned char rings[];
+  const Part<VEC, E> t = {WARP ? int(threadIdx.x & 31) : int(threadIdx.x), WARP ? 32 : int(blockDim.x), p.dim};
+  const int64_t worker = WARP ? int64_t(blockIdx.x) * (THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  if (worker >= p.workers) return;
+  unsigned char* ring = rings + (WARP ? (threadIdx.x >> 5) * kStages * 2 * p.row_bytes : 0);
+  const Stream<T, VEC, E> z = {static_cast<const T*>(p.z), p.z_row, ring, 2 * p.row_bytes};
+  const Stream<T, VEC, E> residual = {static_cast<const T*>(p.residual), p.residual_row, ring + p.row_bytes, 2 * p.row_bytes};
+  const float inv_dim = 1.f / float(p.dim);
+  const int64_t begin = worker * p.rows / p.workers, end = (worker + 1) * p.rows / p.workers;
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < end) z.fetch(t, row, stage), residual.fetch(t, row, stage);
+    copy_commit();
+  };
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = 0.f;
+  for (int i = 0; i < kStages; ++i) fetch(begin + i, i);
+  float c[E], pre[E];
+  if (p.pre) load_part<W, VEC, E>(pre, t, static_cast<const W*>(p.pre));
+  int64_t group = begin / p.rows_per_gate, group_end = (group + 1) * p.rows_per_gate;
+  coefficients<T, W, VEC, E>(c, t, p, group);
+  int stage = 0, side = 0;
+  for (int64_t row = begin; row < end; ++row, side ^= 1) {
+    if (row == group_end) {
+      ++group, group_end += p.rows_per_gate;
+      coefficients<T, W, VEC, E>(c, t, p, group);
     }
-    float rz = 1.f;
-    if (p.post) {
-      float s = 0.f;
+    copy_wait(kStages - 1);
+    float x[E], r[E];
+    z.load(x, t, row, stage);
+    residual.load(r, t, row, stage);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // of z z, r r, r c z, c z c z
 #pragma unroll
-      for (int i = 0; i < E; ++i) s = fmaf(z[i], z[i], s);
-      rz = rsqrtf(row_sum<WARP>(s, scratch[0]) * inv_dim + p.eps);
-      float w[E];
-      load_part<W, VEC, E>(w, p.post, 0, first, width, p.dim);
-#pragma unroll
-      for (int i = 0; i < E; ++i) z[i] *= rz * w[i];
+    for (int i = 0; i < E; ++i) {
+      const float cz = c[i] * x[i];
+      s[0] = fmaf(x[i], x[i], s[0]);
+      s[1] = fmaf(r[i], r[i], s[1]);
+      s[2] = fmaf(r[i], cz, s[2]);
+      s[3] = fmaf(cz, cz, s[3]);
+      x[i] = cz;
     }
-    if (p.gate) {
-      float g[E];
-      load_part<T, VEC, E>(g, p.gate, row / p.rows_per_gate * p.gate_row, first, width, p.dim);
+    row_sums<WARP, 4>(s, scratch[side]);
+    const float rz = p.post ? rsqrtf(fmaf(s[0], inv_dim, p.eps)) : 1.f;
 #pragma unroll
-      for (int i = 0; i < E; ++i) z[i] *= act_of(p.act, g[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = fmaf(p.scale, z[i], o[i]);
-    store_part<T, VEC, E>(p.out, row * p.dim, o, first, width, p.dim);
+    for (int i = 0; i < E; ++i) x[i] = fmaf(rz, x[i], r[i]);
+    store_part<T, VEC, E>(static_cast<T*>(p.out) + row * p.dim, t, x);
     if (p.pre) {
-      float s = 0.f;
+      float so = s[1] + rz * fmaf(rz, s[3], 2.f * s[2]);
+      if (cancelled(so, s[1], rz * rz * s[3])) {
+        float o[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < E; ++i) s = fmaf(o[i], o[i], s);
-      const float ro = rsqrtf(row_sum<WARP>(s, scratch[1]) * inv_dim + p.eps);
-      float w[E];
-      load_part<W, VEC, E>(w, p.pre, 0, first, width, p.dim);
+        for (int i = 0; i < E; ++i) o[0] = fmaf(x[i], x[i], o[0]);
+        row_sums<WARP, 2>(o, again[side]);
+        so = o[0];
+      }
+      const float ro = rsqrtf(fmaf(so, inv_dim, p.eps));
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] *= ro * w[i];
-      store_part<T, VEC, E>(p.normed, row * p.dim, o, first, width, p.dim);
+      for (int i = 0; i < E; ++i) x[i] *= ro * pre[i];
+      store_part<T, VEC, E>(static_cast<T*>(p.normed) + row * p.dim, t, x);
     }
-    if (!WARP && !(p.post && p.pre)) __syncthreads();  // one sum a row: its scratch is used again at once
+    fetch(row + kStages, stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
 }
 
 template <typename T, typename W, int VEC, int E, bool WARP, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 norm_residual_backward_kernel(const NormArgs p) {
-  __shared__ float scratch[4][32];
-  const int first = WARP ? threadIdx.x & 31 : threadIdx.x, width = WARP ? 32 : blockDim.x;
-  const int64_t workers = p.workers;
-  const int64_t worker  = WARP ? int64_t(blockIdx.x) * (THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
-  if (worker >= workers) return;
+  __shared__ float scratch[2][8 * 33], again[2][2][2 * 33];
+  extern __shared__ __align__(16) unsigned char rings[];
+  const Part<VEC, E> t = {WARP ? int(threadIdx.x & 31) : int(threadIdx.x), WARP ? 32 : int(blockDim.x), p.dim};
+  const int64_t worker = WARP ? int64_t(blockIdx.x) * (THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  if (worker >= p.workers) return;
+  unsigned char* ring = rings + (WARP ? (threadIdx.x >> 5) * kStages * 4 * p.row_bytes : 0);
+  const int stage_bytes = 4 * p.row_bytes;
+  const Stream<T, VEC, E> z = {static_cast<const T*>(p.z), p.z_row, ring, stage_bytes};
+  const Stream<T, VEC, E> residual = {static_cast<const T*>(p.pre ? p.residual : nullptr), p.residual_row, ring + p.row_bytes, stage_bytes};
+  const Stream<T, VEC, E> dout = {static_cast<const T*>(p.dout), p.dout_row, ring + 2 * p.row_bytes, stage_bytes};
+  const Stream<T, VEC, E> dnormed = {static_cast<const T*>(p.pre ? p.dnormed : nullptr), p.dnormed_row, ring + 3 * p.row_bytes, stage_bytes};
   const float inv_dim = 1.f / float(p.dim);
-  float dpost[E], dpre[E];
+  auto begin_of = [&](int64_t unit) { return unit / p.slices * p.rows_per_gate + unit % p.slices * p.slice_rows; };
+  const int64_t first_unit = worker * p.units / p.workers, last_unit = (worker + 1) * p.units / p.workers;
+  int64_t end = begin_of(last_unit);  // the worker's rows lie one behind the other
+  if (end > p.rows) end = p.rows;
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < end) z.fetch(t, row, stage), residual.fetch(t, row, stage), dout.fetch(t, row, stage), dnormed.fetch(t, row, stage);
+    copy_commit();
+  };
+  int64_t row = begin_of(first_unit);
 #pragma unroll
-  for (int i = 0; i < E; ++i) dpost[i] = dpre[i] = 0.f;
-  const int64_t unit_end = (worker + 1) * p.units / workers;
-  for (int64_t unit = worker * p.units / workers; unit < unit_end; ++unit) {
-    const int64_t group = unit / p.slices, slice = unit % p.slices;
-    const int64_t begin = group * p.rows_per_gate + slice * p.slice_rows;
-    int64_t end         = begin + p.slice_rows;
-    if (end > (group + 1) * p.rows_per_gate) end = (group + 1) * p.rows_per_gate;
-    float dgate[E];
+  for (int i = 0; i < kStages; ++i) fetch(row + i, i);
+  float c[E], pre[E], dpost[E], dpre[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) dgate[i] = 0.f;
-    for (int64_t row = begin; row < end; ++row) {
-      float z[E], o[E], d[E], du[E];
-      load_part<T, VEC, E>(z, p.z, row * p.z_row, first, width, p.dim);
+  for (int i = 0; i < E; ++i) dpost[i] = dpre[i] = pre[i] = 0.f;
+  if (p.pre) load_part<W, VEC, E>(pre, t, static_cast<const W*>(p.pre));
+  int stage = 0, side = 0;
+  for (int64_t unit = first_unit; unit < last_unit; ++unit) {
+    const int64_t group = unit / p.slices;
+    int64_t unit_end    = begin_of(unit) + p.slice_rows;
+    if (unit_end > (group + 1) * p.rows_per_gate) unit_end = (group + 1) * p.rows_per_gate;
+    coefficients<T, W, VEC, E>(c, t, p, group);
+    float q[E];  // the sum over rows of d zn
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = d[i] = du[i] = 0.f;
-      if (p.pre && p.residual) load_part<T, VEC, E>(o, p.residual, row * p.residual_row, first, width, p.dim);
-      if (p.dout) load_part<T, VEC, E>(d, p.dout, row * p.dout_row, first, width, p.dim);
-      if (p.pre && p.dnormed) load_part<T, VEC, E>(du, p.dnormed, row * p.dnormed_row, first, width, p.dim);
-      float rz = 1.f;
-      if (p.post) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) s = fmaf(z[i], z[i], s);
-        rz = rsqrtf(row_sum<WARP>(s, scratch[0]) * inv_dim + p.eps);
-#pragma unroll
-        for (int i = 0; i < E; ++i) z[i] *= rz;  // z / rms(z) from here on
-      }
-      float post[E], gate[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i) post[i] = gate[i] = 1.f;
-      if (p.post) load_part<W, VEC, E>(post, p.post, 0, first, width, p.dim);
-      if (p.gate) {
-        load_part<T, VEC, E>(gate, p.gate, group * p.gate_row, first, width, p.dim);
-#pragma unroll
-        for (int i = 0; i < E; ++i) gate[i] = act_of(p.act, gate[i]);
-      }
-      if (p.pre) {
-        float pre[E], so = 0.f, sv = 0.f;
-        load_part<W, VEC, E>(pre, p.pre, 0, first, width, p.dim);
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          o[i] = fmaf(p.scale * gate[i], z[i] * post[i], o[i]);
-          so   = fmaf(o[i], o[i], so);
-          sv   = fmaf(du[i] * pre[i], o[i], sv);
-        }
-        const float ro   = rsqrtf(row_sum<WARP>(so, scratch[1]) * inv_dim + p.eps);
-        const float mean = row_sum<WARP>(sv, scratch[2]) * inv_dim * ro;  // of v on
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const float on = o[i] * ro;
-          dpre[i] = fmaf(du[i], on, dpre[i]);
-          d[i]    = fmaf(ro, fmaf(-on, mean, du[i] * pre[i]), d[i]);
-        }
-      }
-      if (p.dresidual) store_part<T, VEC, E>(p.dresidual, row * p.dim, d, first, width, p.dim);
-      float sw = 0.f;
+    for (int i = 0; i < E; ++i) q[i] = 0.f;
+    for (; row < unit_end; ++row, side ^= 1) {
+      copy_wait(kStages - 1);
+      float x[E], r[E], d[E], du[E];
+      z.load(x, t, row, stage);
+      residual.load(r, t, row, stage);
+      dout.load(d, t, row, stage);
+      dnormed.load(du, t, row, stage);
+      // of z z, r r, r c z, c z c z, v r, v c z, c z do
+      float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        d[i] *= p.scale;
-        dgate[i] = fmaf(d[i], z[i] * post[i], dgate[i]);
-        d[i] *= gate[i];  // dn
-        dpost[i] = fmaf(d[i], z[i], dpost[i]);
-        d[i] *= post[i];  // w
-        sw = fmaf(d[i], z[i], sw);
+        const float cz = c[i] * x[i], v = du[i] * pre[i];
+        s[0] = fmaf(x[i], x[i], s[0]);
+        s[1] = fmaf(r[i], r[i], s[1]);
+        s[2] = fmaf(r[i], cz, s[2]);
+        s[3] = fmaf(cz, cz, s[3]);
+        s[4] = fmaf(v, r[i], s[4]);
+        s[5] = fmaf(v, cz, s[5]);
+        s[6] = fmaf(cz, d[i], s[6]);
       }
+      row_sums<WARP, 8>(s, scratch[side]);
+      const float rz = p.post ? rsqrtf(fmaf(s[0], inv_dim, p.eps)) : 1.f;
+      float ro = 0.f, minus_k = 0.f, mean = s[6];  // d = do + ro v + minus_k o;  mean: of c d z, times dim
+      if (p.pre) {
+        float so = s[1] + rz * fmaf(rz, s[3], 2.f * s[2]), vo = fmaf(rz, s[5], s[4]);
+        const bool careful = cancelled(so, s[1], rz * rz * s[3]);
+        if (careful) {
+          float y[2] = {0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const float o = fmaf(rz * c[i], x[i], r[i]);
+            y[0] = fmaf(o, o, y[0]);
+            y[1] = fmaf(du[i] * pre[i], o, y[1]);
+          }
+          row_sums<WARP, 2>(y, again[side][0]);
+          so = y[0], vo = y[1];
+        }
+        ro      = rsqrtf(fmaf(so, inv_dim, p.eps));
+        minus_k = -ro * ro * ro * vo * inv_dim;
+        mean    = s[6] + ro * s[5] + minus_k * fmaf(rz, s[3], s[2]);
+        if (careful) {
+          float y[2] = {0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const float o = fmaf(rz * c[i], x[i], r[i]);
+            y[0] = fmaf(c[i] * x[i], fmaf(minus_k, o, fmaf(ro, du[i] * pre[i], d[i])), y[0]);
+          }
+          row_sums<WARP, 2>(y, again[side][1]);
+          mean = y[0];
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float o = fmaf(rz * c[i], x[i], r[i]);
+          dpre[i] = fmaf(du[i], o * ro, dpre[i]);
+          d[i]    = fmaf(minus_k, o, fmaf(ro, du[i] * pre[i], d[i]));
+        }
+      }
+      if (p.dresidual) store_part<T, VEC, E>(static_cast<T*>(p.dresidual) + row * p.dim, t, d);
+      const float shift = p.post ? -rz * rz * mean * inv_dim : 0.f;  // dz = rz (c d + shift z), rz inside: mean(c d zn) zn
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        q[i] = fmaf(d[i], rz * x[i], q[i]);
+        d[i] = rz * fmaf(shift, x[i], c[i] * d[i]);
+      }
+      store_part<T, VEC, E>(static_cast<T*>(p.dz) + row * p.dim, t, d);
+      fetch(row + kStages, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    // dpost += scale act(gate) q, dgate = scale act'(gate) post q
+    float gate[E];
+    if (p.gate) load_part<T, VEC, E>(gate, t, static_cast<const T*>(p.gate) + group * p.gate_row);
+    if (p.post_parts) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) dpost[i] = fmaf(p.gate ? p.scale * act_of(p.act, gate[i]) : p.scale, q[i], dpost[i]);
+    }
+    if (p.dgate || p.gate_parts) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) q[i] *= p.scale * slope_of(p.act, gate[i]);
       if (p.post) {
-        const float mean = row_sum<WARP>(sw, scratch[3]) * inv_dim;  // of w zn
+        load_part<W, VEC, E>(gate, t, static_cast<const W*>(p.post));
 #pragma unroll
-        for (int i = 0; i < E; ++i) d[i] = rz * fmaf(-z[i], mean, d[i]);
+        for (int i = 0; i < E; ++i) q[i] *= gate[i];
       }
-      store_part<T, VEC, E>(p.dz, row * p.dim, d, first, width, p.dim);
+      if (p.dgate) store_part<T, VEC, E>(static_cast<T*>(p.dgate) + group * p.dim, t, q);
+      if (p.gate_parts) store_part<float, VEC, E>(p.gate_parts + unit * p.dim, t, q);
     }
-    if (p.gate && p.act != kNone) {
-      float gate[E];
-      load_part<T, VEC, E>(gate, p.gate, group * p.gate_row, first, width, p.dim);
-#pragma unroll
-      for (int i = 0; i < E; ++i) dgate[i] *= slope_of(p.act, gate[i]);
-    }
-    if (p.dgate) store_part<T, VEC, E>(p.dgate, group * p.dim, dgate, first, width, p.dim);
-    if (p.gate_parts) store_part<float, VEC, E>(p.gate_parts, unit * p.dim, dgate, first, width, p.dim);
   }
-  if (p.post_parts) store_part<float, VEC, E>(p.post_parts, worker * p.dim, dpost, first, width, p.dim);
-  if (p.pre_parts) store_part<float, VEC, E>(p.pre_parts, worker * p.dim, dpre, first, width, p.dim);
+  if (p.post_parts) store_part<float, VEC, E>(p.post_parts + worker * p.dim, t, dpost);
+  if (p.pre_parts) store_part<float, VEC, E>(p.pre_parts + worker * p.dim, t, dpre);
 }
 
 // out[g][c] = sum over k of parts[g * count + k][c], in a fixed order; blockIdx.y is g over three jobs.
@@ -285,18 +417,45 @@ column_sums_kernel(const Jobs jobs) {
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kMaxDim       = 16384;
-constexpr int kForwardE     = 16;    // elements per thread
-constexpr int kWarpThreads  = 256;   // rows that a warp holds: eight to a block
-constexpr int kBackwardThreads = 148 * 1024;  // of the backward pass: 1024 on each SM
+constexpr int kMaxDim      = 16384;
+constexpr int kWarpThreads = 256;  // rows that a warp holds (up to 256 elements): eight to a block
+constexpr int kWarpDim     = 256;
 
-int warp_dim(int e) { return 32 * e; }
-
-// A row's threads, whole warps.
+// A row's threads, whole warps, for E elements a thread.
 int row_threads(int64_t dim, int e) { return int((dim + e * 32 - 1) / (e * 32) * 32); }
 
-// Elements per thread of the backward pass: it keeps sums for each of them.
-int backward_e(int64_t dim) { return dim <= 512 * 8 ? 8 : 16; }
+// Elements per thread: 8, but not more threads than `most`.
+int elements(int64_t dim, int most) { return dim <= most * 8 ? 8 : 16; }
+
+// Of the backward pass, which needs 100 registers and more: 512 threads for each SM.
+constexpr int kBackwardThreads = 148 * 512;
+
+template <typename K>
+cudaError_t allow_shared(K kernel, bool* configured, int bytes) {
+  const int dev = current_device();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return cudaSuccess;
+}
+constexpr int kMostShared = 216 << 10;
+
+// Launches a kernel whose ring holds kStages rows of `arrays` arrays for each of `rings` rows at a time.
+template <typename K>
+int launch_rows(K kernel, bool* configured, NormArgs p, int elem, int vec, int arrays, int rings, unsigned grid, int threads,
+                cudaStream_t st) {
+  p.row_bytes     = vec > 1 ? (p.dim * elem + 15) / 16 * 16 : 0;
+  const int bytes = kStages * arrays * rings * p.row_bytes;
+  if (allow_shared(kernel, configured, kMostShared) != cudaSuccess) return TCU_ERR_CUDA;
+  kernel<<<grid, threads, bytes, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
+}
+
+// Whether a ring of rows of `arrays` arrays fits into shared memory.
+bool ring_fits(int64_t dim, size_t elem, int arrays) { return kStages * arrays * (dim * int64_t(elem) + 15) / 16 * 16 <= kMostShared; }
 
 bool row_vectors(const void* p, size_t elem, int64_t stride, int vec) {
   return aligned(p, elem * vec < 16 ? elem * vec : 16) && stride % vec == 0;
@@ -317,7 +476,7 @@ struct Cut {
 };
 
 Cut cut_rows(int64_t rows, int64_t dim, int64_t gate_rows) {
-  const int64_t most = kBackwardThreads / row_threads(dim, backward_e(dim));
+  const int64_t most = kBackwardThreads / row_threads(dim, elements(dim, 512));
   const int64_t per  = rows / gate_rows;
   Cut c;
   int64_t slices = gate_rows >= most ? 1 : most / gate_rows;
@@ -367,26 +526,37 @@ int tcu_norm_residual(const tcu_norm_residual_args* g, void* stream) {
     using W = decltype(w);
     constexpr int V = 16 / sizeof(T);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool wide = p.dim % V == 0 && row_vectors(p.z, e, p.z_row, V) && row_vectors(p.residual, e, p.residual_row, V) &&
+    const bool wide = p.dim % V == 0 && ring_fits(p.dim, e, 2) && row_vectors(p.z, e, p.z_row, V) && row_vectors(p.residual, e, p.residual_row, V) &&
                       row_vectors(p.gate, e, p.gate_row, V) && row_vectors(p.post, ew, 0, V) &&
                       row_vectors(p.pre, ew, 0, V) && aligned(p.out, 16) && aligned(p.normed, 16);
-    const bool warp   = p.dim <= warp_dim(kForwardE);
-    const int threads = warp ? kWarpThreads : row_threads(p.dim, kForwardE);
-    const int64_t blocks = warp ? (p.rows + 7) / 8 : p.rows;
-    const int64_t most   = int64_t(sms) * (2048 / threads);
-    const unsigned grid  = unsigned(blocks < most ? blocks : most);
-    if (wide) {
-      if (warp)
-        norm_residual_kernel<T, W, V, kForwardE, true, kWarpThreads><<<grid, threads, 0, st>>>(p);
-      else
-        norm_residual_kernel<T, W, V, kForwardE, false, 1024><<<grid, threads, 0, st>>>(p);
-    } else {
-      if (warp)
-        norm_residual_kernel<T, W, 1, kForwardE, true, kWarpThreads><<<grid, threads, 0, st>>>(p);
-      else
-        norm_residual_kernel<T, W, 1, kForwardE, false, 1024><<<grid, threads, 0, st>>>(p);
-    }
-    return cudaGetLastError() == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
+    auto go = [&](auto vec) -> int {
+      constexpr int VEC = decltype(vec)::value;
+      const int e8 = elements(p.dim, 1024), threads = row_threads(p.dim, e8);
+      if (p.dim <= kWarpDim) {
+        static bool ready[kMaxDevices];
+        p.workers = p.rows < int64_t(sms) * 64 ? p.rows : int64_t(sms) * 64;
+        return launch_rows(norm_residual_kernel<T, W, VEC, 8, true, kWarpThreads, 4>, ready, p, sizeof(T), VEC, 2, 8,
+                           unsigned((p.workers + 7) / 8), kWarpThreads, st);
+      }
+      const int blocks = threads > 768 || e8 == 16 ? 1 : threads > 512 ? 2 : 1536 / threads;  // on an SM
+      p.workers        = p.rows < int64_t(sms) * blocks ? p.rows : int64_t(sms) * blocks;
+      const unsigned grid = unsigned(p.workers);
+      if (e8 == 16) {
+        static bool ready[kMaxDevices];
+        return launch_rows(norm_residual_kernel<T, W, VEC, 16, false, 1024, 1>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
+      }
+      if (threads <= 512) {
+        static bool ready[kMaxDevices];
+        return launch_rows(norm_residual_kernel<T, W, VEC, 8, false, 512, 3>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
+      }
+      if (threads <= 768) {
+        static bool ready[kMaxDevices];
+        return launch_rows(norm_residual_kernel<T, W, VEC, 8, false, 768, 2>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
+      }
+      static bool ready[kMaxDevices];
+      return launch_rows(norm_residual_kernel<T, W, VEC, 8, false, 1024, 1>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
+    };
+    return wide ? go(std::integral_constant<int, V>{}) : go(std::integral_constant<int, 1>{});
   });
 }
 
@@ -444,28 +614,32 @@ int tcu_norm_residual_backward(const tcu_norm_residual_backward_args* g, void* s
     using T = decltype(t);
     using W = decltype(w);
     constexpr int V = 16 / sizeof(T);
-    const bool wide = p.dim % V == 0 && row_vectors(p.z, e, p.z_row, V) && row_vectors(p.residual, e, p.residual_row, V) &&
+    const bool wide = p.dim % V == 0 && ring_fits(p.dim, e, 4) && row_vectors(p.z, e, p.z_row, V) && row_vectors(p.residual, e, p.residual_row, V) &&
                       row_vectors(p.gate, e, p.gate_row, V) && row_vectors(p.dout, e, p.dout_row, V) &&
                       row_vectors(p.dnormed, e, p.dnormed_row, V) && row_vectors(p.post, ew, 0, V) &&
                       row_vectors(p.pre, ew, 0, V) && aligned(p.dz, 16) && aligned(p.dresidual, 16) && aligned(p.dgate, 16);
-    auto go = [&](auto vec) {
+    auto go = [&](auto vec) -> int {
       constexpr int VEC = decltype(vec)::value;
-      if (p.dim <= warp_dim(8)) {
-        const unsigned grid = unsigned((c.workers + 7) / 8);
-        norm_residual_backward_kernel<T, W, VEC, 8, true, kWarpThreads><<<grid, kWarpThreads, 0, st>>>(p);
-      } else if (p.dim <= 512 * 8) {
-        norm_residual_backward_kernel<T, W, VEC, 8, false, 512><<<unsigned(c.workers), row_threads(p.dim, 8), 0, st>>>(p);
-      } else if (p.dim <= 512 * 16) {
-        norm_residual_backward_kernel<T, W, VEC, 16, false, 512><<<unsigned(c.workers), row_threads(p.dim, 16), 0, st>>>(p);
-      } else {
-        norm_residual_backward_kernel<T, W, VEC, 16, false, 1024><<<unsigned(c.workers), row_threads(p.dim, 16), 0, st>>>(p);
+      const int e8 = elements(p.dim, 512), threads = row_threads(p.dim, e8);
+      const unsigned grid = unsigned(c.workers);
+      if (p.dim <= kWarpDim) {
+        static bool ready[kMaxDevices];
+        return launch_rows(norm_residual_backward_kernel<T, W, VEC, 8, true, kWarpThreads>, ready, p, sizeof(T), VEC, 4, 8,
+                           (grid + 7) / 8, kWarpThreads, st);
       }
+      if (e8 == 8) {
+        static bool ready[kMaxDevices];
+        return launch_rows(norm_residual_backward_kernel<T, W, VEC, 8, false, 512>, ready, p, sizeof(T), VEC, 4, 1, grid, threads, st);
+      }
+      if (threads <= 512) {
+        static bool ready[kMaxDevices];
+        return launch_rows(norm_residual_backward_kernel<T, W, VEC, 16, false, 512>, ready, p, sizeof(T), VEC, 4, 1, grid, threads, st);
+      }
+      // (a ring of rows of more than 8192 elements does not fit with four arrays of 32 bits)
+      static bool ready[kMaxDevices];
+      return launch_rows(norm_residual_backward_kernel<T, W, 1, 16, false, 1024>, ready, p, sizeof(T), 1, 4, 1, grid, threads, st);
     };
-    if (wide)
-      go(std::integral_constant<int, V>{});
-    else
-      go(std::integral_constant<int, 1>{});
-    return cudaGetLastError() == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
+    return wide ? go(std::integral_constant<int, V>{}) : go(std::integral_constant<int, 1>{});
   });
   if (err != TCU_OK) return err;
   Jobs jobs{};

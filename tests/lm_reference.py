@@ -125,9 +125,15 @@ def norm_residual(z, residual, post, gate, act, scale, pre, eps, dout=None, dnor
     pre and gate before they are summed over rows are post_rows, pre_rows and gate_rows."""
     dim = z.shape[1]
     chain = 16 + 5 + 6  # a thread's elements, its warp, the block's warps
+    # The sums that come behind the first norm may be put together from sums of products of the inputs and of
+    # 1 / rms(z), 2^n of it: the roundings of each part, and the 25 u of 1 / rms(z), count by the size of the parts.
+    # (Unless they cancel to less than a quarter, when they are summed directly.)
+    parts = (chain + 25 + 8) * U
 
-    def scaled(y):  # y / rms(y) and 1 / rms(y)
+    def scaled(y, size=None):  # y / rms(y) and 1 / rms(y)
         mean = (y * y).sum(1, True, chain) * (1.0 / dim)
+        if size is not None:
+            mean.e = mean.e + parts * torch.minimum(size.sum(1, keepdim=True), 8 * (y.v * y.v).sum(1, keepdim=True)) / dim
         ms = Run(mean.v + eps, mean.e + U * (mean.v + eps))
         r = ms.call(lambda m: m.rsqrt(), 0.51 * (ms.v - ms.e).clamp(min=1e-300) ** -1.5)
         return y * r, r
@@ -146,11 +152,13 @@ def norm_residual(z, residual, post, gate, act, scale, pre, eps, dout=None, dnor
     else:
         g = Run(torch.ones_like(z))
     o = n * g * scale
+    branch = o.v.abs()
+    rest = residual.abs() if residual is not None else torch.zeros_like(z)
     if residual is not None:
         o = o + Run(residual)
     got["out"] = o
     if pre is not None:
-        on, ro = scaled(o)
+        on, ro = scaled(o, (branch + rest) ** 2)
         got["normed"] = on * Run(pre)
     if dout is None:
         return got
@@ -158,6 +166,8 @@ def norm_residual(z, residual, post, gate, act, scale, pre, eps, dout=None, dnor
     if pre is not None:
         v = Run(dnormed) * Run(pre)
         mean = (v * on).sum(1, True, chain + 2) * (1.0 / dim)
+        mean.e = mean.e + parts * (v.v.abs() * (branch + rest)).sum(1, keepdim=True) * ro.v / dim
+        k = (ro.v * mean.v).abs()
         got["pre_rows"] = Run(dnormed) * on
         d = d + ro * (v - on * mean)
     got["dresidual"] = d
@@ -169,6 +179,10 @@ def norm_residual(z, residual, post, gate, act, scale, pre, eps, dout=None, dnor
         got["post_rows"] = dn * zn
         w = dn * Run(post)
         mean = (w * zn).sum(1, True, chain + 2) * (1.0 / dim)
+        size = dout.abs()
+        if pre is not None:
+            size = size + ro.v * v.v.abs() + k * ro.v * (branch + rest)
+        mean.e = mean.e + parts * ((g.v * post * scale).abs() * zn.v.abs() * size).sum(1, keepdim=True) / dim
         got["dz"] = rz * (w - zn * mean)
     else:
         got["dz"] = dn

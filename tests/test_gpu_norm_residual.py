@@ -116,6 +116,18 @@ def test_zero_rows_and_large_values():
     assert bool(out[1].isnan().all()) and not bool(out[[0, 2, 3, 4, 5]].isnan().any())
 
 
+@pytest.mark.parametrize("dim", [100, 512, 1111, 4096])
+def test_branch_that_cancels_the_residual(dim):
+    """The second norm's sum must not be put together from parts that cancel."""
+    import tcu_scope_b200 as tcu
+    s = make(9, dim, F32, F32, 1, 8)
+    z = s["z"].double()
+    n = z / (z.pow(2).mean(1, keepdim=True) + 1e-6).sqrt() * s["post"].double() * s["gate"].double() * 0.75
+    for row, left in enumerate((0.0, 1e-6, 1e-4, 1e-2, 0.1, 0.4, 0.6, 1.0, 2.0)):
+        s["residual"][row] = (-n[row] + left * s["residual"][row].double()).float()
+    check(s, "none", *run(tcu, s, "none"))
+
+
 def test_no_rows():
     import tcu_scope_b200 as tcu
     s = make(1, 48, BF16, F32, 1, 8)
