@@ -427,8 +427,12 @@ int row_threads(int64_t dim, int e) { return int((dim + e * 32 - 1) / (e * 32) *
 // Elements per thread: 8, but not more threads than `most`.
 int elements(int64_t dim, int most) { return dim <= most * 8 ? 8 : 16; }
 
-// Of the backward pass, which needs 100 registers and more: 512 threads for each SM.
-constexpr int kBackwardThreads = 148 * 512;
+// Workers of the backward pass, which needs 100 registers and more: as many as 512 threads on each of the 148 SMs
+// are (a number that leaves some SMs with one more than others takes twice as long: 236 blocks of 320 threads).
+int64_t backward_workers(int64_t dim) {
+  const int threads = dim <= kWarpDim ? 32 : row_threads(dim, elements(dim, 512));
+  return threads > 512 ? 148 : 148 * (512 / threads);
+}
 
 template <typename K>
 cudaError_t allow_shared(K kernel, bool* configured, int bytes) {
@@ -476,7 +480,7 @@ struct Cut {
 };
 
 Cut cut_rows(int64_t rows, int64_t dim, int64_t gate_rows) {
-  const int64_t most = kBackwardThreads / row_threads(dim, elements(dim, 512));
+  const int64_t most = backward_workers(dim);
   const int64_t per  = rows / gate_rows;
   Cut c;
   int64_t slices = gate_rows >= most ? 1 : most / gate_rows;
@@ -531,30 +535,26 @@ int tcu_norm_residual(const tcu_norm_residual_args* g, void* stream) {
                       row_vectors(p.pre, ew, 0, V) && aligned(p.out, 16) && aligned(p.normed, 16);
     auto go = [&](auto vec) -> int {
       constexpr int VEC = decltype(vec)::value;
-      const int e8 = elements(p.dim, 1024), threads = row_threads(p.dim, e8);
       if (p.dim <= kWarpDim) {
         static bool ready[kMaxDevices];
         p.workers = p.rows < int64_t(sms) * 64 ? p.rows : int64_t(sms) * 64;
         return launch_rows(norm_residual_kernel<T, W, VEC, 8, true, kWarpThreads, 4>, ready, p, sizeof(T), VEC, 2, 8,
                            unsigned((p.workers + 7) / 8), kWarpThreads, st);
       }
-      const int blocks = threads > 768 || e8 == 16 ? 1 : threads > 512 ? 2 : 1536 / threads;  // on an SM
+      const int e8 = elements(p.dim, 512), threads = row_threads(p.dim, e8);
+      const int blocks = threads > 512 ? 1 : e8 == 16 ? 1024 / threads : 2048 / threads;  // for an SM
       p.workers        = p.rows < int64_t(sms) * blocks ? p.rows : int64_t(sms) * blocks;
       const unsigned grid = unsigned(p.workers);
-      if (e8 == 16) {
+      if (e8 == 8) {
         static bool ready[kMaxDevices];
-        return launch_rows(norm_residual_kernel<T, W, VEC, 16, false, 1024, 1>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
+        return launch_rows(norm_residual_kernel<T, W, VEC, 8, false, 512, 2>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
       }
       if (threads <= 512) {
         static bool ready[kMaxDevices];
-        return launch_rows(norm_residual_kernel<T, W, VEC, 8, false, 512, 3>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
-      }
-      if (threads <= 768) {
-        static bool ready[kMaxDevices];
-        return launch_rows(norm_residual_kernel<T, W, VEC, 8, false, 768, 2>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
+        return launch_rows(norm_residual_kernel<T, W, VEC, 16, false, 512, 2>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
       }
       static bool ready[kMaxDevices];
-      return launch_rows(norm_residual_kernel<T, W, VEC, 8, false, 1024, 1>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
+      return launch_rows(norm_residual_kernel<T, W, VEC, 16, false, 1024, 1>, ready, p, sizeof(T), VEC, 2, 1, grid, threads, st);
     };
     return wide ? go(std::integral_constant<int, V>{}) : go(std::integral_constant<int, 1>{});
   });

@@ -26,33 +26,44 @@ ACT = {"none": 0, "sigmoid": 1, "silu": 2}
 _INDEX = (torch.int32, torch.int64)
 
 
-def _launch(name: str, layout: struct.Struct, fields, device: torch.device) -> None:
-    """Calls an entry point that takes a struct of 8-byte fields, on the tensors' device."""
-    args = layout.pack(*fields)
-    fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+# The current stream and device as plain numbers: the calls behind torch.cuda.current_stream() and
+# current_device(), which take 2 us more, as long as a small operator runs.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_entries: dict = {}
+
+
+def _launch(name: str, args: bytes, device: torch.device) -> None:
+    """Calls an entry point that takes a struct of 8-byte fields, on the tensors' device and its current stream."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    index = device.index
+    if index == _device_now():
+        status = fn(args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(args, torch.cuda.current_stream(device).cuda_stream)
-    _check(status, name)
+            status = fn(args, _raw_stream(index))
+    if status:
+        _check(status, name)
 
 
 def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _inputs(device: torch.device, **tensors: torch.Tensor | None) -> None:
+def _inputs(device: torch.device, names: tuple, tensors: tuple) -> None:
     """What every input has to be: on the device of the first one, and not recorded by autograd."""
     if device.type != "cuda":
         raise RuntimeError("input must be a CUDA tensor: there is no CPU path in this library")
-    for name, t in tensors.items():
+    for i, t in enumerate(tensors):
         if t is None:
             continue
         if t.device != device:
-            raise RuntimeError(f"{name} is on {t.device}, the other tensors on {device}")
+            raise RuntimeError(f"{names[i]} is on {t.device}, the other tensors on {device}")
         if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} requires a gradient, which autograd would not get: call under "
+            raise RuntimeError(f"{names[i]} requires a gradient, which autograd would not get: call under "
                                "torch.no_grad() and use the operator's backward function")
 
 
@@ -68,6 +79,13 @@ def _result(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype, device
     if t.device != device or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
     return t
+
+
+def _result_like(t: torch.Tensor | None, name: str, x: torch.Tensor) -> torch.Tensor:
+    """The caller's output tensor, checked, or a new one, of x's shape and type."""
+    if t is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return _result(t, name, x.shape, x.dtype, x.device)
 
 
 def _like(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype) -> None:
@@ -142,21 +160,21 @@ def linear_scan(a: torch.Tensor, x: torch.Tensor, gate: str = "decay", h0: torch
     states: from :func:`linear_scan_states`, for :func:`linear_scan_backward`.
     """
     device = x.device
-    _inputs(device, x=x, a=a, h0=h0, offsets=offsets, states=states)
+    _inputs(device, ("x", "a", "h0", "offsets", "states"), (x, a, h0, offsets, states))
     batch, tokens, dim = _scan_shape(a, x, gate, offsets)
     _like(h0, "h0", (batch, dim), torch.float32)
     clear = out is None
-    h = _result(out, "out", x.shape, x.dtype, device)
+    h = _result_like(out, "out", x)
     last = _result(last, "last", (batch, dim), torch.float32, device)
     if states is not None:
         rows = _lib.load().tcu_linear_scan_states_rows(batch, tokens, 0 if offsets is None else 1)
         _like(states, "states", (rows, dim), torch.float32)
     if offsets is not None and batch == 0:
         return (h.zero_() if clear else h), last
-    _launch("tcu_linear_scan", _SCAN,
-            (_ptr(a), _ptr(x), _ptr(h), _ptr(h0), _ptr(last), _ptr(states), _ptr(offsets), batch, tokens, dim,
-             *_strides(a), *_strides(x), GATE[gate], _TYPE[a.dtype], _TYPE[x.dtype],
-             offsets is not None and offsets.dtype == torch.int64, clear), device)
+    _launch("tcu_linear_scan", _SCAN.pack(
+        _ptr(a), _ptr(x), _ptr(h), _ptr(h0), _ptr(last), _ptr(states), _ptr(offsets), batch, tokens, dim,
+        *_strides(a), *_strides(x), GATE[gate], _TYPE[a.dtype], _TYPE[x.dtype],
+        offsets is not None and offsets.dtype == torch.int64, clear), device)
     return h, last
 
 
@@ -171,7 +189,7 @@ def linear_scan_backward(dh: torch.Tensor | None, a: torch.Tensor, x: torch.Tens
     Rows outside all sequences have gradient 0 in new tensors and are left as they were in the caller's.
     """
     device = x.device
-    _inputs(device, x=x, a=a, dh=dh, states=states, dlast=dlast, offsets=offsets)
+    _inputs(device, ("x", "a", "dh", "states", "dlast", "offsets"), (x, a, dh, states, dlast, offsets))
     batch, tokens, dim = _scan_shape(a, x, gate, offsets)
     if dh is not None:
         if dh.shape != x.shape or dh.dtype != x.dtype:
@@ -183,15 +201,15 @@ def linear_scan_backward(dh: torch.Tensor | None, a: torch.Tensor, x: torch.Tens
     if offsets is not None and (da is None) != (dx is None):
         raise ValueError("with offsets, pass both da and dx or neither")
     clear = da is None
-    da = _result(da, "da", a.shape, a.dtype, device)
-    dx = _result(dx, "dx", x.shape, x.dtype, device)
+    da = _result_like(da, "da", a)
+    dx = _result_like(dx, "dx", x)
     dh0 = _result(dh0, "dh0", (batch, dim), torch.float32, device)
     if offsets is not None and batch == 0:
         return (da.zero_(), dx.zero_(), dh0) if clear else (da, dx, dh0)
-    _launch("tcu_linear_scan_backward", _SCAN_BACKWARD,
-            (_ptr(dh), _ptr(a), _ptr(x), _ptr(states), _ptr(dlast), _ptr(da), _ptr(dx), _ptr(dh0), _ptr(offsets),
-             batch, tokens, dim, *_strides(dh), *_strides(a), *_strides(x), GATE[gate], _TYPE[a.dtype],
-             _TYPE[x.dtype], offsets is not None and offsets.dtype == torch.int64, clear), device)
+    _launch("tcu_linear_scan_backward", _SCAN_BACKWARD.pack(
+        _ptr(dh), _ptr(a), _ptr(x), _ptr(states), _ptr(dlast), _ptr(da), _ptr(dx), _ptr(dh0), _ptr(offsets),
+        batch, tokens, dim, *_strides(dh), *_strides(a), *_strides(x), GATE[gate], _TYPE[a.dtype],
+        _TYPE[x.dtype], offsets is not None and offsets.dtype == torch.int64, clear), device)
     return da, dx, dh0
 
 
@@ -205,7 +223,7 @@ def linear_scan_step(a: torch.Tensor, x: torch.Tensor, state: torch.Tensor, gate
     and for a slot that an earlier row names.
     """
     device = x.device
-    _inputs(device, x=x, a=a, state=state, slots=slots)
+    _inputs(device, ("x", "a", "state", "slots"), (x, a, state, slots))
     if x.dim() != 2 or a.shape != x.shape:
         raise ValueError("a and x must both be (batch, dim)")
     if x.dtype not in _TYPE or a.dtype not in (x.dtype, torch.float32):
@@ -223,12 +241,12 @@ def linear_scan_step(a: torch.Tensor, x: torch.Tensor, state: torch.Tensor, gate
     elif slots.dtype not in _INDEX or tuple(slots.shape) != (batch,) or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int32 or int64 tensor of batch values")
     clear = out is None
-    h = _result(out, "out", x.shape, x.dtype, device)
+    h = _result_like(out, "out", x)
     if batch and dim:
-        _launch("tcu_linear_scan_step", _STEP,
-                (_ptr(a), _ptr(x), _ptr(h), _ptr(state), _ptr(slots), batch, state.size(0), dim, a.stride(0),
-                 x.stride(0), GATE[gate], _TYPE[a.dtype], _TYPE[x.dtype],
-                 slots is not None and slots.dtype == torch.int64, clear), device)
+        _launch("tcu_linear_scan_step", _STEP.pack(
+            _ptr(a), _ptr(x), _ptr(h), _ptr(state), _ptr(slots), batch, state.size(0), dim, a.stride(0),
+            x.stride(0), GATE[gate], _TYPE[a.dtype], _TYPE[x.dtype],
+            slots is not None and slots.dtype == torch.int64, clear), device)
     return h
 
 
@@ -285,6 +303,8 @@ def _norm_arguments(z, residual, post_weight, gate, gate_act, pre_weight):
         if gate.dtype != z.dtype or gate.dim() < 1 or gate.size(-1) != dim:
             raise ValueError("gate must have z's type and last dimension")
         gate_rows = gate.numel() // dim
+        if gate_rows == 1 and gate.dim() == 1:
+            return rows, dim, 1, w_type
         lead, of = tuple(gate.shape[:-1]), tuple(z.shape[:-1])
         fits = lead == () or (len(of) == 1 and len(lead) == 1 and gate_rows > 0 and rows % gate_rows == 0) or \
             any(lead == of[:k] + (1,) * (len(of) - k) for k in range(len(of) + 1))
@@ -313,19 +333,19 @@ def norm_residual(z: torch.Tensor, residual: torch.Tensor | None = None, *,
     ``out`` may be z or residual themselves, ``normed`` z, if they are contiguous.
     """
     device = z.device
-    _inputs(device, z=z, residual=residual, post_weight=post_weight, gate=gate, pre_weight=pre_weight)
+    _inputs(device, ("z", "residual", "post_weight", "gate", "pre_weight"), (z, residual, post_weight, gate, pre_weight))
     rows, dim, gate_rows, w_type = _norm_arguments(z, residual, post_weight, gate, gate_act, pre_weight)
-    out = _result(out, "out", z.shape, z.dtype, device)
+    out = _result_like(out, "out", z)
     if pre_weight is not None:
-        normed = _result(normed, "normed", z.shape, z.dtype, device)
+        normed = _result_like(normed, "normed", z)
     elif normed is not None:
         raise ValueError("normed needs pre_weight")
     if rows:
-        _launch("tcu_norm_residual", _NORM,
-                (_ptr(z), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight), _ptr(out), _ptr(normed),
-                 rows, dim, gate_rows, _row_stride(z, "z"), _row_stride(residual, "residual"),
-                 _row_stride(gate, "gate") if gate_rows > 1 else 0, ACT[gate_act], _TYPE[z.dtype], _TYPE[w_type],
-                 scale, eps), device)
+        _launch("tcu_norm_residual", _NORM.pack(
+            _ptr(z), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight), _ptr(out), _ptr(normed),
+            rows, dim, gate_rows, _row_stride(z, "z"), _row_stride(residual, "residual"),
+            _row_stride(gate, "gate") if gate_rows > 1 else 0, ACT[gate_act], _TYPE[z.dtype], _TYPE[w_type],
+            scale, eps), device)
     return out, normed
 
 
@@ -342,34 +362,33 @@ def norm_residual_backward(dout: torch.Tensor | None, dnormed: torch.Tensor | No
     ``dresidual`` may be dout itself; ``dz`` may be z, dnormed, or, if dresidual is not, dout.
     """
     device = z.device
-    _inputs(device, z=z, residual=residual, post_weight=post_weight, gate=gate, pre_weight=pre_weight, dout=dout,
-            dnormed=dnormed, workspace=workspace)
+    _inputs(device, ("z", "residual", "post_weight", "gate", "pre_weight", "dout", "dnormed", "workspace"), (z, residual, post_weight, gate, pre_weight, dout, dnormed, workspace))
     rows, dim, gate_rows, w_type = _norm_arguments(z, residual, post_weight, gate, gate_act, pre_weight)
     for name, t in (("dout", dout), ("dnormed", dnormed)):
         if t is not None and (t.shape != z.shape or t.dtype != z.dtype):
             raise ValueError(f"{name} must have the shape and type of z")
     if dnormed is not None and pre_weight is None:
         raise ValueError("dnormed needs pre_weight")
-    dz = _result(dz, "dz", z.shape, z.dtype, device)
+    dz = _result_like(dz, "dz", z)
     if residual is not None:
-        dresidual = _result(dresidual, "dresidual", z.shape, z.dtype, device)
+        dresidual = _result_like(dresidual, "dresidual", z)
     elif dresidual is not None:
         raise ValueError("dresidual needs residual")
     dpost = None if post_weight is None else torch.empty_like(post_weight)
     dpre = None if pre_weight is None else torch.empty_like(pre_weight)
-    dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=device)
+    dgate = None if gate is None else _result_like(None, "dgate", gate)
     need = _lib.load().tcu_norm_residual_workspace_bytes(rows, dim, gate_rows)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     elif not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _launch("tcu_norm_residual_backward", _NORM_BACKWARD,
-            (_ptr(dout), _ptr(dnormed), _ptr(z), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight),
-             _ptr(dz), _ptr(dresidual), _ptr(dpost), _ptr(dgate), _ptr(dpre), _ptr(workspace),
-             workspace.numel() * workspace.element_size(), rows, dim, gate_rows, _row_stride(dout, "dout"),
-             _row_stride(dnormed, "dnormed"), _row_stride(z, "z"), _row_stride(residual, "residual"),
-             _row_stride(gate, "gate") if gate_rows > 1 else 0, ACT[gate_act], _TYPE[z.dtype], _TYPE[w_type], scale,
-             eps), device)
+    _launch("tcu_norm_residual_backward", _NORM_BACKWARD.pack(
+        _ptr(dout), _ptr(dnormed), _ptr(z), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight),
+        _ptr(dz), _ptr(dresidual), _ptr(dpost), _ptr(dgate), _ptr(dpre), _ptr(workspace),
+        workspace.numel() * workspace.element_size(), rows, dim, gate_rows, _row_stride(dout, "dout"),
+        _row_stride(dnormed, "dnormed"), _row_stride(z, "z"), _row_stride(residual, "residual"),
+        _row_stride(gate, "gate") if gate_rows > 1 else 0, ACT[gate_act], _TYPE[z.dtype], _TYPE[w_type], scale,
+        eps), device)
     return NormGradients(dz, dresidual, dpost, dgate, dpre)
 
 
@@ -414,21 +433,21 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     3 of :func:`device_error`, has one whose target is out of range.
     """
     device = logits.device
-    _inputs(device, logits=logits, targets=targets)
+    _inputs(device, ("logits", "targets"), (logits, targets))
     rows, vocab, stride = _logits_rows(logits, targets)
     if top > vocab:
         raise ValueError("top is more than the vocabulary")
     lead = logits.shape[:-1]
-    sums = torch.empty((3, *lead), dtype=torch.float32, device=device)
-    lse, entropy = sums[0], sums[1]
-    logprob = sums[2] if targets is not None else None
+    lse, entropy, logprob = torch.empty((3, *lead), dtype=torch.float32, device=device).unbind(0)
+    if targets is None:
+        logprob = None
     top_logprob = torch.empty((*lead, top), dtype=torch.float32, device=device) if top else None
     top_index = torch.empty((*lead, top), dtype=torch.int64, device=device) if top else None
     if rows:
-        _launch("tcu_token_logprobs", _LOGPROBS,
-                (_ptr(logits), _ptr(targets), _ptr(logprob), _ptr(entropy), _ptr(lse), _ptr(top_logprob),
-                 _ptr(top_index), rows, vocab, stride, top, ignore_index, _TYPE[logits.dtype],
-                 targets is not None and targets.dtype == torch.int64), device)
+        _launch("tcu_token_logprobs", _LOGPROBS.pack(
+            _ptr(logits), _ptr(targets), _ptr(logprob), _ptr(entropy), _ptr(lse), _ptr(top_logprob),
+            _ptr(top_index), rows, vocab, stride, top, ignore_index, _TYPE[logits.dtype],
+            targets is not None and targets.dtype == torch.int64), device)
     return TokenLogprobs(logprob, entropy, lse, top_logprob, top_index)
 
 
@@ -442,16 +461,16 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor | None, 
     ``out`` may be the logits themselves, if they are contiguous.
     """
     device = logits.device
-    _inputs(device, logits=logits, targets=targets, lse=lse, entropy=entropy, dlogprob=dlogprob, dentropy=dentropy)
+    _inputs(device, ("logits", "targets", "lse", "entropy", "dlogprob", "dentropy"), (logits, targets, lse, entropy, dlogprob, dentropy))
     rows, vocab, stride = _logits_rows(logits, targets)
     for name, t in (("lse", lse), ("entropy", entropy), ("dlogprob", dlogprob), ("dentropy", dentropy)):
         _like(t, name, logits.shape[:-1], torch.float32)
     if (dlogprob is not None and targets is None) or (dentropy is not None and entropy is None):
         raise ValueError("dlogprob needs targets, dentropy needs entropy")
-    out = _result(out, "out", logits.shape, logits.dtype, device)
+    out = _result_like(out, "out", logits)
     if rows:
-        _launch("tcu_token_logprobs_backward", _LOGPROBS_BACKWARD,
-                (_ptr(logits), _ptr(targets), _ptr(lse), _ptr(entropy), _ptr(dlogprob), _ptr(dentropy), _ptr(out),
-                 rows, vocab, stride, ignore_index, _TYPE[logits.dtype],
-                 targets is not None and targets.dtype == torch.int64), device)
+        _launch("tcu_token_logprobs_backward", _LOGPROBS_BACKWARD.pack(
+            _ptr(logits), _ptr(targets), _ptr(lse), _ptr(entropy), _ptr(dlogprob), _ptr(dentropy), _ptr(out),
+            rows, vocab, stride, ignore_index, _TYPE[logits.dtype],
+            targets is not None and targets.dtype == torch.int64), device)
     return out
