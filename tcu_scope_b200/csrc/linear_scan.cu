@@ -86,9 +86,10 @@ struct Sequence {
   int64_t length;
 };
 
+template <bool PACKED>
 __device__ __forceinline__ Sequence sequence_of(const ScanArgs& p, int64_t b) {
   Sequence s;
-  if (p.offsets == nullptr) {
+  if (!PACKED) {
     s.length = p.tokens;
     s.a      = b * p.a_batch;
     s.x      = b * p.x_batch;
@@ -109,6 +110,32 @@ __device__ __forceinline__ Sequence sequence_of(const ScanArgs& p, int64_t b) {
   s.out    = first * p.dim;
   s.chunk  = first / kSpacing + b;  // distinct: a sequence has at most length / kSpacing + 1 states
   return s;
+}
+
+// Packed sequences of many lengths: blocks of the longest begin first, so that the others fill in beside them.
+// Returns the sequence that `rank` of the others come before; up to kRankedBatch sequences.
+constexpr int kRankedBatch = 96;  // 1 KB more of shared memory and clusters lose their second block on an SM
+
+__device__ __forceinline__ int sequence_of_rank(const void* offsets, bool wide, int batch, int rank) {
+  __shared__ int64_t length[kRankedBatch];
+  __shared__ int found;
+  for (int i = threadIdx.x; i < batch; i += blockDim.x)
+    length[i] = load_index(offsets, i + 1, wide) - load_index(offsets, i, wide);
+  __syncthreads();
+  for (int i = threadIdx.x; i < batch; i += blockDim.x) {
+    const int64_t mine = length[i];
+    int before = 0;
+    for (int j = 0; j < batch; ++j) before += length[j] > mine || (length[j] == mine && j < i);
+    if (before == rank) found = i;
+  }
+  __syncthreads();
+  return found;
+}
+
+template <bool PACKED>
+__device__ __forceinline__ int64_t sequence_at(const ScanArgs& p, int64_t place) {
+  if (!PACKED || p.batch > kRankedBatch) return place;
+  return sequence_of_rank(p.offsets, p.wide, int(p.batch), int(place));
 }
 
 // ------------------------------------------------------------------ the ring
@@ -226,9 +253,10 @@ struct Place {
   int64_t b, first, ch;  // sequence, the block's first channel, the lane's
   int left, count;       // channels of the block from `first`; of the lane: above 0, above 1
 };
+template <bool PACKED>
 __device__ __forceinline__ Place place_of(const ScanArgs& p, int64_t group) {
   Place w;
-  w.b     = group / p.columns;
+  w.b     = sequence_at<PACKED>(p, group / p.columns);
   w.first = group % p.columns * kWidth, w.ch = w.first + (threadIdx.x & 31) * 2;
   w.left  = p.dim - w.first < kWidth ? int(p.dim - w.first) : kWidth;
   w.count = w.left - int(threadIdx.x & 31) * 2;
@@ -282,7 +310,8 @@ __device__ __forceinline__ float2 join_maps(Maps& m, const Map& mine, float2& st
 }
 
 // ------------------------------------------------------------------ forward
-template <typename T, typename A, int GATE>
+// PACKED: the sequences lie one behind the other, by p.offsets.
+template <typename T, typename A, int GATE, bool PACKED>
 __global__ void __launch_bounds__(kMaxWarps * 32, kForwardBlocks)
 linear_scan_kernel(const ScanArgs p) {
   constexpr int kRows = kJoinedRows;
@@ -292,11 +321,11 @@ linear_scan_kernel(const ScanArgs p) {
   const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t group = blockIdx.x / parts;
-  const int64_t b     = group / p.columns;
+  const int64_t b     = sequence_at<PACKED>(p, group / p.columns);
   const int64_t first = (group % p.columns) * kWidth, ch = first + lane * 2;
   const int left = p.dim - first < kWidth ? int(p.dim - first) : kWidth;  // channels of the block
   const int count = left - lane * 2;                                      // of the lane: above 0, above 1
-  const Sequence s = sequence_of(p, b);
+  const Sequence s = sequence_of<PACKED>(p, b);
   const A* a = static_cast<const A*>(p.a) + s.a + first;
   const T* x = static_cast<const T*>(p.x) + s.x + first;
   T* out     = static_cast<T*>(p.h) + s.out + ch;
@@ -358,7 +387,7 @@ linear_scan_kernel(const ScanArgs p) {
     fetch(row + p.stages * step, stage);
     stage = stage + 1 == p.stages ? 0 : stage + 1;
   }
-  if (p.clear_rest) clear_rest<T>(p, static_cast<T*>(p.h) + ch, b, count, part, parts);
+  if (PACKED && p.clear_rest) clear_rest<T>(p, static_cast<T*>(p.h) + ch, b, count, part, parts);
   if (p.last && part == 0 && warp == 0) {
     float* last = p.last + b * p.dim + ch;
     if (count > 0) last[0] = state.x;
@@ -368,7 +397,7 @@ linear_scan_kernel(const ScanArgs p) {
 
 // ------------------------------------------------------------------ backward
 // JOINED: the warps of a block and the blocks of a cluster share a sequence's time; else a block is one warp.
-template <typename T, typename A, int GATE, bool JOINED>
+template <typename T, typename A, int GATE, bool JOINED, bool PACKED>
 __global__ void __launch_bounds__(JOINED ? kMaxWarps * 32 : 32, JOINED ? kBackwardBlocks<GATE> : 1)
 linear_scan_backward_kernel(const ScanArgs p) {
   constexpr int kRows = JOINED ? kJoinedRows : kLoneRows;
@@ -377,8 +406,8 @@ linear_scan_backward_kernel(const ScanArgs p) {
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = JOINED ? int(cluster.num_blocks()) : 1, part = JOINED ? int(cluster.block_rank()) : 0;
   const int warp = JOINED ? threadIdx.x >> 5 : 0, warps = JOINED ? blockDim.x >> 5 : 1;
-  const Place w    = place_of(p, blockIdx.x / parts);
-  const Sequence s = sequence_of(p, w.b);
+  const Place w    = place_of<PACKED>(p, blockIdx.x / parts);
+  const Sequence s = sequence_of<PACKED>(p, w.b);
   const A* a  = static_cast<const A*>(p.a) + s.a + w.first;
   const T* x  = static_cast<const T*>(p.x) + s.x + w.first;
   const T* dy = static_cast<const T*>(p.dh) + s.dh + w.first;
@@ -457,9 +486,9 @@ linear_scan_backward_kernel(const ScanArgs p) {
     }
     float2 before[kRows];
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) {
+    for (int n0 = 0; n0 < kParts; ++n0) {
 #pragma unroll
-      for (int i = part * kSpacing; i < (part + 1) * kSpacing; i += kGroup) {
+      for (int i = n0 * kSpacing; i < (n0 + 1) * kSpacing; i += kGroup) {
         float2 f[kGroup], rest[kGroup], u[kGroup];
         gates_at(i, f, rest);
 #pragma unroll
@@ -468,7 +497,7 @@ linear_scan_backward_kernel(const ScanArgs p) {
           if constexpr (GATE == TCU_GATE_SIGMOID) u[k] = mul2(rest[k], u[k]);
         }
 #pragma unroll
-        for (int k = 0; k < kGroup; ++k) before[i + k] = h[part], h[part] = fma2(f[k], h[part], u[k]);
+        for (int k = 0; k < kGroup; ++k) before[i + k] = h[n0], h[n0] = fma2(f[k], h[n0], u[k]);
       }
     }
 #pragma unroll
@@ -497,7 +526,7 @@ linear_scan_backward_kernel(const ScanArgs p) {
     fetch(row - p.stages * step, stage);
     stage = stage + 1 == p.stages ? 0 : stage + 1;
   }
-  if (p.clear_rest) {
+  if (PACKED && p.clear_rest) {
     clear_rest<A>(p, static_cast<A*>(p.da) + w.ch, w.b, w.count, part, parts);
     clear_rest<T>(p, static_cast<T*>(p.dx) + w.ch, w.b, w.count, part, parts);
   }
@@ -629,7 +658,10 @@ cudaError_t launch_scan(ScanArgs args, int row_bytes, int blocks, int sms, cudaS
   };
   if (Lone == Joined || (groups < int64_t(kLoneColumns) * sms && each > kLoneRows)) {
     warps = kMaxWarps;
-    while (warps > 2 && (2 * (bytes_of(2) + 17 * 1024) > (226 << 10) || (warps > 4 && groups > int64_t(sms) * fit())))
+    // (packed sequences need not all fit at once: few are long)
+    const bool at_once = !args.offsets || args.batch > kRankedBatch;
+    while (warps > 2 && (2 * (bytes_of(2) + 17 * 1024) > (226 << 10) ||
+                         (warps > 4 && at_once && groups > int64_t(sms) * fit())))
       warps /= 2;
     while (parts < kMaxCluster && groups * parts < sms && each > int64_t(parts) * warps * kJoinedRows) parts *= 2;
   }
@@ -695,8 +727,12 @@ int tcu_linear_scan(const tcu_linear_scan_args* g, void* stream) {
     using T = decltype(t);
     using A = decltype(a);
     constexpr int G = decltype(gate)::value;
-    return launch_scan<linear_scan_kernel<T, A, G>, linear_scan_kernel<T, A, G>>(
-        p, kWidth * int(sizeof(A) + sizeof(T)), kForwardBlocks, sms, static_cast<cudaStream_t>(stream));
+    auto go = [&](auto packed) {
+      constexpr auto kernel = linear_scan_kernel<T, A, G, decltype(packed)::value>;
+      return launch_scan<kernel, kernel>(p, kWidth * int(sizeof(A) + sizeof(T)), kForwardBlocks, sms,
+                                         static_cast<cudaStream_t>(stream));
+    };
+    return p.offsets ? go(std::true_type{}) : go(std::false_type{});
   });
   return err == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
 }
@@ -730,8 +766,12 @@ int tcu_linear_scan_backward(const tcu_linear_scan_backward_args* g, void* strea
     using T = decltype(t);
     using A = decltype(a);
     constexpr int G = decltype(gate)::value;
-    return launch_scan<linear_scan_backward_kernel<T, A, G, false>, linear_scan_backward_kernel<T, A, G, true>>(
-        p, kWidth * int(sizeof(A) + 2 * sizeof(T)), kBackwardBlocks<G>, sms, static_cast<cudaStream_t>(stream));
+    auto go = [&](auto packed) {
+      constexpr bool P = decltype(packed)::value;
+      return launch_scan<linear_scan_backward_kernel<T, A, G, false, P>, linear_scan_backward_kernel<T, A, G, true, P>>(
+          p, kWidth * int(sizeof(A) + 2 * sizeof(T)), kBackwardBlocks<G>, sms, static_cast<cudaStream_t>(stream));
+    };
+    return p.offsets ? go(std::true_type{}) : go(std::false_type{});
   });
   return err == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
 }
