@@ -39,7 +39,8 @@ def _newer_than(target: str, sources: list[str]) -> bool:
 
 # The translation units of the library.  capi.cu includes every kernel of the reductions and scans
 # (fp16 inputs), capi_bf16.cu the same sources for bf16 inputs.
-UNITS = ["capi.cu", "capi_bf16.cu", "linear_scan.cu", "norm_residual.cu", "token_logprobs.cu"]
+UNITS = ["capi.cu", "capi_bf16.cu", "linear_scan.cu", "linear_scan_f16.cu", "linear_scan_bf16.cu", "linear_scan_f32.cu",
+         "norm_residual.cu", "token_logprobs.cu"]
 
 
 def _sources() -> list[str]:

@@ -153,9 +153,9 @@ def linear_scan(a: torch.Tensor, x: torch.Tensor, gate: str = "decay", h0: torch
     (batch, dim), the states behind the last ones (may be h0 itself).
 
     With ``offsets`` (batch + 1 values, int32 or int64, on the device) x and a are (tokens, dim) and sequence b is their rows
-    ``offsets[b] ... offsets[b+1]-1``.  An empty sequence leaves its state as it is.  Rows outside all
-    sequences are 0 in a new ``h`` and are left as they were in ``out``.  A sequence whose offsets decrease or
-    pass the end counts as empty and raises bit 3 of :func:`device_error`.
+    ``offsets[b] ... offsets[b+1]-1``.  An empty sequence leaves its state as it is.  Rows before the first and behind
+    the last sequence are 0 in a new ``h`` and are left as they were in ``out``.  A sequence whose offsets decrease or
+    pass the end counts as empty and raises bit 3 of :func:`device_error`; its rows are not written.
 
     states: from :func:`linear_scan_states`, for :func:`linear_scan_backward`.
     """
@@ -186,7 +186,8 @@ def linear_scan_backward(dh: torch.Tensor | None, a: torch.Tensor, x: torch.Tens
 
     dh: the gradient of h (x's shape and type; None: zero); dlast: that of ``last`` (None: zero); a, x, gate and
     offsets: as in the forward call, states: as it left them.  da and dx have the types of a and x, dh0 is float32.
-    Rows outside all sequences have gradient 0 in new tensors and are left as they were in the caller's.
+    Rows before the first and behind the last sequence have gradient 0 in new tensors and are left as they were in the
+    caller's.
     """
     device = x.device
     _inputs(device, ("x", "a", "dh", "states", "dlast", "offsets"), (x, a, dh, states, dlast, offsets))
