@@ -329,7 +329,7 @@ typedef enum { TCU_TYPE_F16 = 0, TCU_TYPE_F32 = 1, TCU_TYPE_BF16 = 2 } tcu_type;
  * Gates are meant to have |f| <= 1: the product of up to 1024 of them in a
  * row must stay within float32.
  *
- * x, a: `batch` sequences of `tokens` rows of `dim` elements; h: contiguous.
+ * x, a: `batch` sequences of `tokens` rows of `dim` (up to 2^21) elements; h: contiguous.
  * With `offsets` (batch + 1 values, not decreasing, 32- or 64-bit) the
  * sequences lie one behind the other instead, sequence b being the rows
  * offsets[b] ... offsets[b+1]-1 of `tokens` rows in all (batch strides
@@ -408,6 +408,7 @@ int tcu_linear_scan_step(const tcu_linear_scan_step_args* args, void* stream);
  *     out = residual + scale * act(gate) * n        (residual 0, act(gate) 1 if not given)
  *     normed = out / rms(out) * pre_weight          (only with pre_weight)
  * with rms(y) = sqrt(mean(y^2) + eps), and out not rounded before it is normed.
+ * (Sums of squares of a row must stay within float32.)
  * gate: gate_rows rows, each for rows / gate_rows consecutive rows (1: one
  * learned vector; rows: a gate for every element); gate_rows divides rows.
  * type: of z, residual, gate, out and normed; weight_type: that type or
@@ -437,7 +438,8 @@ int tcu_norm_residual(const tcu_norm_residual_args* args, void* stream);
  * sums over rows are made in a fixed order.  dresidual may be dout's buffer,
  * dz may be z's, dout's (if that is not dresidual too) or dnormed's, if that is
  * contiguous.  The workspace is 16-byte aligned, of
- * tcu_norm_residual_workspace_bytes(), and needs no initialisation.
+ * tcu_norm_residual_workspace_bytes(), needs no initialisation, and must not be
+ * shared by calls that can run at the same time.
  */
 typedef struct {
   const void* dout;        /* may be NULL */

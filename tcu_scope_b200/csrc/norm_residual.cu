@@ -20,6 +20,10 @@
 //
 // Bound by HBM: 4 arrays forward, 6 backward.  Rows come through a ring in shared memory, each thread copying (cp.async)
 // what it will read itself: nothing is waited for but a thread's own copies and the one meeting.
+// Measured, of the copy bandwidth: forward 16384 x 4096 bf16 105 us (77 %), 65536 x 256 81 % (a warp a row, no meeting),
+// bound by the instructions a row takes; gradient 225 us (54 %), of which its seven sums take 62: it needs 127 registers, so
+// that one block of 512 threads is on an SM and nothing runs while that meets.  (Two meetings forward and four
+// backward took 129 and 509 us; pairs of floats in one instruction 131 and 237.)
 #include <type_traits>
 
 #include "lm_common.cuh"

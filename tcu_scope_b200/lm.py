@@ -360,7 +360,8 @@ def norm_residual_backward(dout: torch.Tensor | None, dnormed: torch.Tensor | No
 
     The other arguments are those of the forward call.  Each gradient has the shape and type of what it is the
     gradient of; those of weights and of a gate that rows share are summed over the rows in a fixed order.
-    ``dresidual`` may be dout itself; ``dz`` may be z, dnormed, or, if dresidual is not, dout.
+    ``dresidual`` may be dout itself; ``dz`` may be z, dnormed, or, if dresidual is not, dout.  workspace: bytes
+    (tcu_norm_residual_workspace_bytes), not shared by calls that can run at the same time; default: a new one.
     """
     device = z.device
     _inputs(device, ("z", "residual", "post_weight", "gate", "pre_weight", "dout", "dnormed", "workspace"), (z, residual, post_weight, gate, pre_weight, dout, dnormed, workspace))
