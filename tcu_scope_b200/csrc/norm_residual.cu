@@ -173,9 +173,10 @@ __device__ __forceinline__ void coefficients(float (&c)[E], const Part<VEC, E>& 
   }
 }
 
-// Whether sum o^2, of terms of this size, has lost digits.
+// Whether sum o^2, of terms of this size, has lost digits, or a part left float32 (which o itself need not do).
 __device__ __forceinline__ bool cancelled(float sum, float residual_part, float branch_part) {
-  return sum < 0.25f * (residual_part + branch_part);
+  const float parts = residual_part + branch_part;
+  return !(sum >= 0.25f * parts) || parts == INFINITY;
 }
 
 template <typename T, typename W, int VEC, int E, bool WARP, int THREADS, int BLOCKS>

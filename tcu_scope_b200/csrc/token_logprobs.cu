@@ -15,7 +15,7 @@
 // A row is read by the P blocks of a cluster, P > 1 where there are few rows, which join their sums
 // and lists in shared memory of the first.  Bound by HBM: one read forward, a read and a write backward.
 // Measured, bf16: 4096 x 128000 174 us (92 % of the copy bandwidth) without, 211 us with 8 alternatives: 83 % of the issue slots
-// are taken, by 9 instructions an element and the exponentials' unit at 16 a cycle; gradient of 2048 x 100003 170 us (74 %).
+// are taken, by 9 instructions an element and the exponentials' unit at 16 a cycle; gradient of 2048 x 100003 141 us (88 %).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -546,9 +546,10 @@ __device__ __noinline__ Sums block_row_sums(const Row<T>& row, Sums* scratch) {
   return join_warp((threadIdx.x & 31) < kBackThreads / 32 ? scratch[threadIdx.x & 31] : Sums());
 }
 
-// dx_j = dlp ([j = target] - p_j) - dH p_j (log p_j + H), H the entropy.
+// dx_j = dlp ([j = target] - p_j) - dH p_j (log p_j + H), H the entropy.  Six blocks on an SM (40 registers) hide one
+// another's loads: 2048 x 100003 bf16 141 us, 153 with five, 170 with the four that 61 registers leave room for.
 template <typename T>
-__global__ void __launch_bounds__(kBackThreads)
+__global__ void __launch_bounds__(kBackThreads, 6)
 token_logprobs_backward_kernel(const LogprobArgs p) {
   __shared__ Sums scratch[kBackThreads / 32];
   constexpr int V   = kVec<T>;

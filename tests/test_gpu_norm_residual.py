@@ -128,6 +128,18 @@ def test_branch_that_cancels_the_residual(dim):
     check(s, "none", *run(tcu, s, "none"))
 
 
+@pytest.mark.parametrize("dim", [200, 1000])
+def test_parts_beyond_float32(dim):
+    """Products of large rows and weights leave float32 although the row's sum of squares and all results do not."""
+    import tcu_scope_b200 as tcu
+    s = make(5, dim, F32, F32, 1, 8)
+    s["z"][1] *= 1e17
+    s["z"][3] *= 1e17
+    s["residual"][3] = 0
+    s["post"] *= 1000
+    check(s, "none", *run(tcu, s, "none"))
+
+
 def test_no_rows():
     import tcu_scope_b200 as tcu
     s = make(1, 48, BF16, F32, 1, 8)
