@@ -530,9 +530,11 @@ token_logprobs_kernel(const LogprobArgs p) {
 constexpr int kBackThreads = 256;
 
 // Above this size lse has lost more than 2^-16 of log p to its own rounding, and the gradient goes by the
-// row's largest element and the sum against it instead, for which every block reads the row once more.
+// row's largest element and the sum against it instead, for which the row is read once more.  Such a row is one
+// block's: the gradient may lie over the logits, and no block may write while another still sums.
 constexpr float kExactLse = 256.f;
 
+// The sums of a row, in every thread; no thread returns before all have read their elements.
 template <typename T>
 __device__ __noinline__ Sums block_row_sums(const Row<T>& row, Sums* scratch) {
   Sums a;
@@ -574,18 +576,21 @@ token_logprobs_backward_kernel(const LogprobArgs p) {
   }
   // log2 p = (x - ref) log2(e) - shift
   float ref = empty ? 0.f : lse, shift = 0.f;
+  const int64_t block = blockIdx.x % p.blocks_per_row;
+  int64_t vectors     = p.vectors_per_block;
   if (!empty && fabsf(lse) > kExactLse) {
+    if (block != 0) return;
     const Sums a = block_row_sums<T>(row, scratch);
-    ref   = a.ref;
-    shift = log2f(a.s);
+    ref     = a.ref;
+    shift   = log2f(a.s);
+    vectors = row.vectors;
   }
   const float c0 = -fmaf(dent, entropy, dlp), c1 = -dent * kLn2;
   // Elements 200 (and up to 32 for the rounding to T) below lse have p = 0; raised to that, neither they
   // nor -inf make log2 p so large that 0 times it is not 0.
   const bool near   = fabsf(ref) < 1e4f && !empty;
   const float floor = ref - 200.f;
-  const int begin = int(blockIdx.x % p.blocks_per_row * p.vectors_per_block);
-  const int end   = begin + int(p.vectors_per_block) < row.vectors ? begin + int(p.vectors_per_block) : row.vectors;
+  const int begin = int(block * vectors), end = begin + int(vectors) < row.vectors ? begin + int(vectors) : row.vectors;
   for (int v0 = begin + threadIdx.x; v0 < end; v0 += kBackThreads * kUnroll) {
     Block16<T> raw[kUnroll];
 #pragma unroll

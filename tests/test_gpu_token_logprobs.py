@@ -188,6 +188,30 @@ def test_gradient_over_the_logits(vocab):
     assert torch.equal(tcu.token_logprobs_backward(x, t, got.lse, got.entropy, dlogprob=one, dentropy=one, out=out), want)
 
 
+@pytest.mark.parametrize("kind", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(3, 20011), (64, 20016), (5, 100003), (150, 100000)])
+def test_gradient_over_the_logits_of_rows_far_from_zero(kind, rows, vocab):
+    """Rows whose lse has lost digits are summed once more for the gradient: all of a row is read before any
+    of it is overwritten, however many blocks a row of ordinary size has."""
+    import tcu_scope_b200 as tcu
+    x, t = make(rows, vocab, kind, rows + vocab)
+    x[0] += 3000
+    x[2:-1] -= 20000 if kind == F16 else 1e6  # the last row and row 1 stay as they are
+    x[2::3] += 19000 if kind == F16 else 1e6 - 1000
+    got = tcu.token_logprobs(x, t)
+    assert int((got.lse.abs() > 256).sum()) >= rows - 2
+    g = torch.Generator().manual_seed(3)
+    dlp, dent = torch.randn(rows, generator=g).cuda(), torch.randn(rows, generator=g).cuda()
+    want = tcu.token_logprobs_backward(x, t, got.lse, got.entropy, dlogprob=dlp, dentropy=dent)
+    few = slice(0, 4)
+    bound = ref.token_logprobs(x[few].double().cpu(), t[few].cpu(), 0, dlp[few].double().cpu(), dent[few].double().cpu())
+    ref.assert_within(want[few], *bound["dlogits"], "dlogits")
+    for _ in range(3):
+        over = x.clone()
+        tcu.token_logprobs_backward(over, t, got.lse, got.entropy, dlogprob=dlp, dentropy=dent, out=over)
+        assert torch.equal(over, want)
+
+
 def test_gradient_against_differences():
     import tcu_scope_b200 as tcu
     x, t = make(3, 11, F32, 8, spread=1.0)
