@@ -307,7 +307,9 @@ norm_residual_backward_kernel(const NormArgs p) {
       }
       row_sums<WARP, 8>(s, scratch[side]);
       const float rz = p.post ? rsqrtf(fmaf(s[0], inv_dim, p.eps)) : 1.f;
-      float ro = 0.f, minus_k = 0.f, mean = s[6];  // d = do + ro v + minus_k o;  mean: of c d z, times dim
+      // d = do + ro (v - m on), on = ro o, m = mean(v on);  mean: of c d z, times dim.  (Only one ro is multiplied at a
+      // time: ro^2 and ro^3 leave float32 for rows whose sum of squares does not.)
+      float ro = 0.f, m = 0.f, mean = s[6];
       if (p.pre) {
         float so = s[1] + rz * fmaf(rz, s[3], 2.f * s[2]), vo = fmaf(rz, s[5], s[4]);
         const bool careful = cancelled(so, s[1], rz * rz * s[3]);
@@ -322,28 +324,28 @@ norm_residual_backward_kernel(const NormArgs p) {
           row_sums<WARP, 2>(y, again[side][0]);
           so = y[0], vo = y[1];
         }
-        ro      = rsqrtf(fmaf(so, inv_dim, p.eps));
-        minus_k = -ro * ro * ro * vo * inv_dim;
-        mean    = s[6] + ro * s[5] + minus_k * fmaf(rz, s[3], s[2]);
+        ro   = rsqrtf(fmaf(so, inv_dim, p.eps));
+        m    = ro * vo * inv_dim;
+        mean = fmaf(ro, fmaf(-m, ro * fmaf(rz, s[3], s[2]), s[5]), s[6]);
         if (careful) {
           float y[2] = {0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < E; ++i) {
             const float o = fmaf(rz * c[i], x[i], r[i]);
-            y[0] = fmaf(c[i] * x[i], fmaf(minus_k, o, fmaf(ro, du[i] * pre[i], d[i])), y[0]);
+            y[0] = fmaf(c[i] * x[i], fmaf(ro, fmaf(-m, o * ro, du[i] * pre[i]), d[i]), y[0]);
           }
           row_sums<WARP, 2>(y, again[side][1]);
           mean = y[0];
         }
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          const float o = fmaf(rz * c[i], x[i], r[i]);
-          dpre[i] = fmaf(du[i], o * ro, dpre[i]);
-          d[i]    = fmaf(minus_k, o, fmaf(ro, du[i] * pre[i], d[i]));
+          const float on = fmaf(rz * c[i], x[i], r[i]) * ro;
+          dpre[i] = fmaf(du[i], on, dpre[i]);
+          d[i]    = fmaf(ro, fmaf(-m, on, du[i] * pre[i]), d[i]);
         }
       }
       if (p.dresidual) store_part<T, VEC, E>(static_cast<T*>(p.dresidual) + row * p.dim, t, d);
-      const float shift = p.post ? -rz * rz * mean * inv_dim : 0.f;  // dz = rz (c d + shift z), rz inside: mean(c d zn) zn
+      const float shift = p.post ? -(rz * mean * inv_dim) * rz : 0.f;  // dz = rz (c d + shift z), rz inside: mean(c d zn) zn
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         q[i] = fmaf(d[i], rz * x[i], q[i]);

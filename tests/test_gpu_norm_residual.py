@@ -140,6 +140,25 @@ def test_parts_beyond_float32(dim):
     check(s, "none", *run(tcu, s, "none"))
 
 
+@pytest.mark.parametrize("kind", [BF16, F32])
+@pytest.mark.parametrize("dim", [200, 1000, 4096])
+@pytest.mark.parametrize("post", [False, True])
+def test_gradient_of_rows_of_any_size(kind, dim, post):
+    """Rows whose 1 / rms has a square or a cube beyond float32, while the sum of squares is not."""
+    import tcu_scope_b200 as tcu
+    for size, eps in ((1e13, 1e-6), (1e15, 1e-6), (1e17, 1e-6), (1e-14, 0.0), (1e-17, 0.0)):
+        for plain in (True, False):  # without a residual, and with one that sets the size of `out` where z is normed
+            s = make(4, dim, kind, F32, 0 if plain else 1, 8, residual=not plain, post=post)
+            s["z"] *= size / 3
+            if not plain:
+                s["residual"] *= size / 3
+            zero = {**s, "dout": torch.zeros_like(s["z"])}
+            none = run(tcu, {**s, "dout": None}, "none", eps=eps)
+            check(zero, "none", *none, eps=eps)
+            s["dout"] *= 1 / size  # as large as what comes through the norm
+            check(s, "none", *run(tcu, s, "none", eps=eps), eps=eps)
+
+
 def test_no_rows():
     import tcu_scope_b200 as tcu
     s = make(1, 48, BF16, F32, 1, 8)
