@@ -335,7 +335,8 @@ typedef enum { TCU_TYPE_F16 = 0, TCU_TYPE_F32 = 1, TCU_TYPE_BF16 = 2 } tcu_type;
  * offsets[b] ... offsets[b+1]-1 of `tokens` rows in all (batch strides
  * are not used); rows before the first and behind the last sequence are left as
  * they were, or become 0 where clear_rest is not 0, and a sequence whose offsets are out of range or decrease counts as
- * empty.  a_type: the type of x, or TCU_TYPE_F32.
+ * empty.  Of sequences that then share rows or lie in another order than their
+ * numbers at most one is not empty, always the same.  a_type: the type of x, or TCU_TYPE_F32.
  * h0, last: batch x dim floats; last (may be h0) receives the state behind
  * each sequence's last row, h0's if the sequence is empty.
  * states: NULL, or tcu_linear_scan_states_rows() x dim floats that

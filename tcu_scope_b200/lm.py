@@ -155,7 +155,8 @@ def linear_scan(a: torch.Tensor, x: torch.Tensor, gate: str = "decay", h0: torch
     With ``offsets`` (batch + 1 values, int32 or int64, on the device) x and a are (tokens, dim) and sequence b is their rows
     ``offsets[b] ... offsets[b+1]-1``.  An empty sequence leaves its state as it is.  Rows before the first and behind
     the last sequence are 0 in a new ``h`` and are left as they were in ``out``.  A sequence whose offsets decrease or
-    pass the end counts as empty and raises bit 3 of :func:`device_error`; its rows are not written.
+    pass the end counts as empty and raises bit 3 of :func:`device_error`; its rows are not written.  So do, but for one
+    of them, sequences that then share rows or lie in another order than their numbers.
 
     states: from :func:`linear_scan_states`, for :func:`linear_scan_backward`.
     """

@@ -199,6 +199,61 @@ def test_wrong_indices_are_left_out_and_reported():
     ref.assert_within(h[5], *want["last"], "h")
 
 
+def offsets_that_decrease():
+    """(tokens, offsets) with sequences that share rows, or (the last) states."""
+    even = list(range(0, 1207, 6))  # 201 sequences of 6 rows
+    def changed(**at):
+        return [at.get(f"o{i}", v) for i, v in enumerate(even)]
+    return [(600, [0, 300, 100, 600]), (600, [0, 50, 120, 60, 400, 600]), (600, [200, 600, 0, 400, 300, 500]),
+            (1206, changed(o57=5000)), (1206, changed(o57=-9, o126=1300)), (1206, changed(o60=0)),
+            (1206, changed(o133=700, o140=650)), (1206, changed(o3=1000, o150=30)), (1206, even[::-1]),
+            (688, [672, 688] + list(range(0, 641, 16)))]
+
+
+@pytest.mark.parametrize("case", range(10))
+@pytest.mark.parametrize("dim", [64, 136])
+def test_sequences_that_share_rows(case, dim):
+    """A sequence that is in order with all others runs; of those that share rows or are out of order at most one
+    does, the same one every time, forward and backward; the rest count as empty."""
+    import tcu_scope_b200 as tcu
+    tokens, offsets = offsets_that_decrease()[case]
+    batch = len(offsets) - 1
+    a, x, n = inputs("decay", (tokens, dim), F32, BF16, case)
+    h0, dlast, dh = n(batch, dim).cuda(), n(batch, dim).cuda(), n(tokens, dim).to(BF16).cuda()
+    at = torch.tensor(offsets, dtype=torch.int64).cuda()
+
+    def run():
+        states = tcu.linear_scan_states(x, at)
+        h, last = tcu.linear_scan(a, x, h0=h0, offsets=at, states=states, out=torch.full_like(x, 7.0))
+        da, dx, dh0 = tcu.linear_scan_backward(dh, a, x, states, dlast=dlast, offsets=at, da=torch.full_like(a, 7.0),
+                                               dx=torch.full_like(x, 7.0))
+        return dict(h=h, da=da, dx=dx, last=last, dh0=dh0)
+
+    got = run()
+    assert tcu.device_error() == 8
+    for _ in range(3):
+        again = run()
+        assert all(torch.equal(got[k], again[k]) for k in got)
+    tcu.device_error()
+    well = [b for b in range(batch) if 0 <= offsets[b] < offsets[b + 1] <= tokens]
+    owner = [None] * tokens
+    cpu = lambda t: t.double().cpu()  # noqa: E731
+    for b in range(batch):
+        i, j = offsets[b], offsets[b + 1]
+        if torch.equal(got["last"][b], h0[b]):
+            assert torch.equal(got["dh0"][b], dlast[b])
+            assert b not in well or any(offsets[k + 1] > i if k < b else offsets[k] < j for k in well if k != b), b
+            continue
+        assert b in well and owner[i:j] == [None] * (j - i), b
+        owner[i:j] = [b] * (j - i)
+        want = ref.linear_scan("decay", cpu(a[i:j]), cpu(x[i:j]), cpu(h0[b]), cpu(dh[i:j]), cpu(dlast[b]))
+        check({k: v[b] if k in ("last", "dh0") else v[i:j] for k, v in got.items()}, want, b)
+    free = torch.tensor([o is None for o in owner]).cuda()
+    for k in ("h", "da", "dx"):
+        assert bool((got[k][free] == 7).all())
+    assert bool(free.all()) == (case == 8)  # something runs, unless nothing can
+
+
 def test_overflowing_products_do_not_spoil_a_zero_state():
     """Gates above 1 whose product leaves float32 while the state is 0, and gates of 0."""
     import tcu_scope_b200 as tcu
