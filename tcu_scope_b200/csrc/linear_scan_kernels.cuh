@@ -137,8 +137,8 @@ __device__ __forceinline__ bool search_finds(const ScanArgs& p, uint32_t b, int6
 // More sequences than kRankedBatch are not all compared: those that the search finds (all, where no offset decreases) are in
 // order among themselves, and of the others those run that are in order with all.  By all threads of a block, when its
 // first rows are on their way, and through shared memory: values that the compiler does not know to be one for the
-// block make the gradient's loop spill.  (bf16, forward + backward, and without the search: 4000 sequences of 10 x 1024 359 + 275
-// us, 315 + 250; 300 of 67 x 2048 77 + 114, 72 + 110; 97 of 206 x 2048 63 + 138, 60 + 136.)
+// block make the gradient's loop spill.  (bf16, forward + backward, and without the search: 4000 sequences of 10 x 1024 359 + 272
+// us, 312 + 249; 300 of 67 x 2048 75 + 107, 72 + 110; 97 of 206 x 2048 62 + 129, 59 + 136.)
 __device__ __forceinline__ void leave_out(const ScanArgs& p, int64_t b, int& left_out) {
   if (p.batch > kRankedBatch) {
     if (threadIdx.x < 32) {
@@ -244,20 +244,36 @@ __device__ __forceinline__ float2 load_pair(const float* p, int count) {
   return make_float2(count > 0 ? p[0] : 0.f, count > 1 ? p[1] : 0.f);
 }
 
-// Rows that no sequence holds, of the channels of this block: those before the first sequence and
-// behind the last one.
+// Rows that no sequence holds: those before the first sequence and behind the last one, which the blocks of these
+// two (b) clear.  Where offsets decrease other sequences may lie there: only what is before or behind all counts.  By all
+// threads of a block.
+struct Rest {
+  int64_t before, behind;  // rows 0 ... before-1 and behind ... tokens-1
+};
+__device__ __forceinline__ Rest rest_of(const ScanArgs& p, int64_t b) {
+  Rest rest = {b == 0 ? load_index(p.offsets, 0, p.wide) : 0, b == p.batch - 1 ? load_index(p.offsets, p.batch, p.wide) : p.tokens};
+  if (rest.before <= 0 && rest.behind >= p.tokens) return {0, p.tokens};
+  __shared__ long long ends[2];
+  if (threadIdx.x == 0) ends[0] = p.tokens, ends[1] = 0;
+  __syncthreads();
+  int64_t low = p.tokens, high = 0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < p.batch; i += blockDim.x) {
+    const int64_t f = load_index(p.offsets, i, p.wide), e = load_index(p.offsets, i + 1, p.wide);
+    if (f >= 0 && f < e && e <= p.tokens) low = f < low ? f : low, high = e > high ? e : high;
+  }
+  atomicMin(&ends[0], low), atomicMax(&ends[1], high);
+  __syncthreads();
+  low = ends[0], high = ends[1];
+  return {rest.before < low ? rest.before : low, rest.behind > high ? rest.behind : high};
+}
+
+// Clears them, of the channels of this block.
 template <typename T>
-__device__ __forceinline__ void clear_rest(const ScanArgs& p, T* out, int64_t b, int count, int part, int parts) {
+__device__ __forceinline__ void clear_rest(const ScanArgs& p, T* out, const Rest& rest, int count, int part, int parts) {
   const int warp = part * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = parts * (blockDim.x >> 5);
-  if (b == 0) {
-    const int64_t first = load_index(p.offsets, 0, p.wide);
-    for (int64_t r = warp; r < first && r < p.tokens; r += warps) store_pair<T>(out + r * p.dim, make_float2(0.f, 0.f), count, p.pairs);
-  }
-  if (b == p.batch - 1) {
-    const int64_t end = load_index(p.offsets, p.batch, p.wide);
-    for (int64_t r = (end < 0 ? 0 : end) + warp; r < p.tokens; r += warps)
-      store_pair<T>(out + r * p.dim, make_float2(0.f, 0.f), count, p.pairs);
-  }
+  for (int64_t r = warp; r < rest.before; r += warps) store_pair<T>(out + r * p.dim, make_float2(0.f, 0.f), count, p.pairs);
+  for (int64_t r = rest.behind + warp; r < p.tokens; r += warps) store_pair<T>(out + r * p.dim, make_float2(0.f, 0.f), count, p.pairs);
 }
 
 // ------------------------------------------------------------------ maps
@@ -413,7 +429,7 @@ linear_scan_kernel(const ScanArgs p) {
     fetch(row + p.stages * step, stage);
     stage = stage + 1 == p.stages ? 0 : stage + 1;
   }
-  if (PACKED && p.clear_rest) clear_rest<T>(p, static_cast<T*>(p.h) + ch, b, count, part, parts);
+  if (PACKED && p.clear_rest && (b == 0 || b == p.batch - 1)) clear_rest<T>(p, static_cast<T*>(p.h) + ch, rest_of(p, b), count, part, parts);
   if (p.last && part == 0 && warp == 0) {
     float* last = p.last + b * p.dim + ch;
     if (count > 0) last[0] = state.x;
@@ -554,9 +570,10 @@ linear_scan_backward_kernel(const ScanArgs p) {
     fetch(row - p.stages * step, stage);
     stage = stage + 1 == p.stages ? 0 : stage + 1;
   }
-  if (PACKED && p.clear_rest) {
-    clear_rest<A>(p, static_cast<A*>(p.da) + w.ch, w.b, w.count, part, parts);
-    clear_rest<T>(p, static_cast<T*>(p.dx) + w.ch, w.b, w.count, part, parts);
+  if (PACKED && p.clear_rest && (w.b == 0 || w.b == p.batch - 1)) {
+    const Rest rest = rest_of(p, w.b);
+    clear_rest<A>(p, static_cast<A*>(p.da) + w.ch, rest, w.count, part, parts);
+    clear_rest<T>(p, static_cast<T*>(p.dx) + w.ch, rest, w.count, part, parts);
   }
   if (p.dh0 && part == 0 && warp == 0) {
     float* dh0 = p.dh0 + w.b * p.dim + w.ch;

@@ -254,6 +254,38 @@ def test_sequences_that_share_rows(case, dim):
     assert bool(free.all()) == (case == 8)  # something runs, unless nothing can
 
 
+@pytest.mark.parametrize("tokens,offsets", [
+    (6, [0, 6, 2]), (6, [5, 0, 6]), (500, [0, 400, 100]), (500, [450, 20, 480]), (500, [300, 320, 100, 130, 420, 60]),
+    (500, [-4, 30, 90]), (500, [10, 30, 600]), (500, [700, 800]), (500, [480, 490, -3]),
+    (700, [690] + [7 * i for i in range(1, 99)] + [3]), (700, [695, 699] + [7 * i for i in range(1, 99)] + [3])])
+@pytest.mark.parametrize("dim", [64, 200])
+def test_cleared_rows_are_no_sequences(tokens, offsets, dim):
+    """New outputs have zeros before the first and behind the last sequence; where offsets decrease, rows of a
+    sequence that lies there all the same are not among them."""
+    import tcu_scope_b200 as tcu
+    batch = len(offsets) - 1
+    a, x, n = inputs("decay", (tokens, dim), F32, BF16, tokens)
+    h0, dlast, dh = n(batch, dim).cuda(), n(batch, dim).cuda(), n(tokens, dim).to(BF16).cuda()
+    at = torch.tensor(offsets, dtype=torch.int32).cuda()
+    states = tcu.linear_scan_states(x, at)
+    h2, last2 = tcu.linear_scan(a, x, h0=h0, offsets=at, out=torch.full_like(x, 7.0), states=states)
+    da2, dx2, dh02 = tcu.linear_scan_backward(dh, a, x, states, dlast=dlast, offsets=at, da=torch.full_like(a, 7.0),
+                                              dx=torch.full_like(x, 7.0))
+    well = [(i, j) for i, j in zip(offsets, offsets[1:]) if 0 <= i < j <= tokens]
+    for _ in range(5):
+        h, last = tcu.linear_scan(a, x, h0=h0, offsets=at)
+        da, dx, dh0 = tcu.linear_scan_backward(dh, a, x, states, dlast=dlast, offsets=at)
+        assert torch.equal(last, last2) and torch.equal(dh0, dh02)
+        for new, old in ((h, h2), (da, da2), (dx, dx2)):
+            for i, j in well:
+                if not bool((old[i:j] == 7).all()):  # it ran
+                    assert torch.equal(new[i:j], old[i:j])
+            before = max(0, min([offsets[0], tokens] + [i for i, _ in well]))
+            behind = max([offsets[-1], 0] + [j for _, j in well])
+            assert bool((new[:before] == 0).all()) and bool((new[behind:] == 0).all())
+    assert tcu.device_error() in ((0, 8) if tokens == 700 else (8,))
+
+
 def test_overflowing_products_do_not_spoil_a_zero_state():
     """Gates above 1 whose product leaves float32 while the state is 0, and gates of 0."""
     import tcu_scope_b200 as tcu
