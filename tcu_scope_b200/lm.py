@@ -6,7 +6,8 @@ probabilities of given tokens (sums of exponentials of rows) with entropy and be
 Like the other operators these take CUDA tensors, call the C ABI on the current stream of the
 tensors' device and return at once.  They are plain functions: autograd does not record them, so a tensor
 that requires a gradient is refused while autograd records (call under ``torch.no_grad()`` or inside a
-``torch.autograd.Function``), and each has a function for its gradient beside it.  An input may be a view
+``torch.autograd.Function``), and one with a tangent of forward-mode autograd is, too; each operator has a function for its
+gradient beside it.  An input may be a view
 with any strides as long as the elements of a row (the last dimension) lie side by side; outputs that
 the caller passes are contiguous and do not overlap other arguments except where it says so.
 """
@@ -31,6 +32,7 @@ _INDEX = (torch.int32, torch.int64)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_forward_ad = torch.autograd.forward_ad
 _entries: dict = {}
 
 
@@ -57,9 +59,13 @@ def _inputs(device: torch.device, names: tuple, tensors: tuple) -> None:
     """What every input has to be: on the device of the first one, and not recorded by autograd."""
     if device.type != "cuda":
         raise RuntimeError("input must be a CUDA tensor: there is no CPU path in this library")
+    duals = getattr(_forward_ad, "_current_level", 0) >= 0  # tensors can have tangents
     for i, t in enumerate(tensors):
         if t is None:
             continue
+        if duals and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{names[i]} has a tangent, which forward-mode autograd would lose: unpack it, or call inside a "
+                               "torch.autograd.Function with a jvp")
         if t.device != device:
             raise RuntimeError(f"{names[i]} is on {t.device}, the other tensors on {device}")
         if t.requires_grad and torch.is_grad_enabled():

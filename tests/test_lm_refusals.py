@@ -101,6 +101,68 @@ def test_cpu_tensors_are_refused(built_library):
         tcu.linear_scan_step(x[0], x[0], x[0])
 
 
+def test_tangents_are_refused(built_library):
+    """Forward-mode autograd would lose them; inside a Function with a jvp of its own they are not there."""
+    import torch.autograd.forward_ad as fw
+    import tcu_scope_b200.lm as lm
+    x, i, cuda = torch.ones(3), torch.zeros(3, dtype=torch.int32), torch.device("cuda", 0)
+
+    class Here:  # the CPU under the name of a GPU
+        type = "cuda"
+
+        def __ne__(self, other):
+            return other != torch.device("cpu")
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(x):
+            lm._inputs(Here(), ("x",), (x,))
+            return 2 * x
+
+        @staticmethod
+        def setup_context(ctx, inputs, output):
+            pass
+
+        @staticmethod
+        def jvp(ctx, t):
+            return 2 * t
+
+    with fw.dual_level():
+        dual = fw.make_dual(x, x)
+        for t in (dual, dual[1:]):
+            for names, tensors in ((("x",), (t,)), (("x", "a"), (t, None))):
+                with pytest.raises(RuntimeError, match="tangent"):
+                    lm._inputs(cuda, names, tensors)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                lm._inputs(cuda, ("x",), (t,))
+        for t in (x, i, fw.unpack_dual(dual).primal):
+            with pytest.raises(RuntimeError, match="cpu"):
+                lm._inputs(cuda, ("x",), (t,))
+        assert torch.equal(fw.unpack_dual(Twice.apply(dual)).tangent, 2 * x)
+
+
+@pytest.mark.gpu
+def test_every_operator_refuses_tangents():
+    import torch.autograd.forward_ad as fw
+    import tcu_scope_b200 as tcu
+    x, w, s = torch.ones(2, 4, 8, device="cuda"), torch.ones(8, device="cuda"), torch.ones(4, 8, device="cuda")
+    states, at, t = tcu.linear_scan_states(x), torch.tensor([0, 4], device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    one = torch.ones(4, device="cuda")
+    with fw.dual_level():
+        dual = lambda v: fw.make_dual(v, torch.ones_like(v))  # noqa: E731
+        for call in (lambda: tcu.linear_scan(x, dual(x)), lambda: tcu.linear_scan(dual(x), x),
+                     lambda: tcu.linear_scan(s, s, h0=dual(w[None]), offsets=at),
+                     lambda: tcu.linear_scan_backward(dual(x), x, x, states), lambda: tcu.linear_scan_step(s, dual(s), s.clone()),
+                     lambda: tcu.linear_scan_step(s, s, dual(s.clone())), lambda: tcu.norm_residual(dual(x), pre_weight=w),
+                     lambda: tcu.norm_residual(x, pre_weight=dual(w)), lambda: tcu.norm_residual(x, dual(x)),
+                     lambda: tcu.norm_residual_backward(dual(x), None, x), lambda: tcu.token_logprobs(dual(s), t),
+                     lambda: tcu.token_logprobs_backward(s, t, one, dlogprob=dual(one))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        h, last = tcu.linear_scan(s, s, h0=w[None], offsets=at)  # tensors without one are taken
+        assert float(last[0, 0]) == 5
+
+
 @pytest.mark.gpu
 def test_linear_scan_python_refusals():
     import tcu_scope_b200 as tcu
