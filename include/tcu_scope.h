@@ -496,6 +496,8 @@ int tcu_token_logprobs(const tcu_token_logprobs_args* args, void* stream);
  * the lse and entropy of the forward call, dlogits (contiguous, the type of the
  * logits; may be their buffer if that is contiguous).  Rows whose target counts
  * for nothing have no part of dlogprob; a row of -inf has gradient 0.
+ * Probabilities go by lse, whose rounding to 32 bits is their relative error;
+ * above |lse| of 32 (TCU_TYPE_F32) or 256 the row is summed once more instead.
  */
 typedef struct {
   const void* logits;

@@ -467,6 +467,8 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor | None, 
     """The gradient of the logits of :func:`token_logprobs`, from those of ``logprob`` and ``entropy`` (None: zero).
 
     lse and entropy: as the forward call returned them (entropy is wanted with dentropy, targets with dlogprob).
+    Probabilities go by lse, whose rounding is their relative error (at most 2^-20 for float32 logits); rows whose |lse| is above
+    32 (256 for 16-bit logits) are summed once more instead.
     ``out`` may be the logits themselves, if they are contiguous.
     """
     device = logits.device

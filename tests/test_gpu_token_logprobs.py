@@ -212,6 +212,28 @@ def test_gradient_over_the_logits_of_rows_far_from_zero(kind, rows, vocab):
         assert torch.equal(over, want)
 
 
+@pytest.mark.parametrize("vocab", [2, 5, 64, 5000, 40000])
+def test_gradient_of_equal_logits_far_from_zero(vocab):
+    """All p are 1 / vocab, whatever the logits are.  Up to |lse| of 32 lse is off by half its step (2^-20) and its own
+    error, above it log2 s by 2 ulp (4 u log2 vocab) and the exponential by 4 u; one product and, at the target, a sum."""
+    import math
+
+    import tcu_scope_b200 as tcu
+    values = [0.0, 3.7, 20.3, 31.9, 33.3, 40.1, 77.7, 100.3, 150.9, 200.1, 255.4, 900.7, -21.2, -90.7, -200.3, -255.9]
+    x = torch.tensor(values).cuda()[:, None].expand(len(values), vocab).contiguous()
+    t = torch.full((len(values),), vocab - 1).cuda()
+    got = tcu.token_logprobs(x, t)
+    d = tcu.token_logprobs_backward(x, t, got.lse, got.entropy, dlogprob=torch.ones(len(values)).cuda()).double().cpu()
+    u, p = 2.0 ** -24, 1.0 / vocab
+    far = [v for v, lse in enumerate(got.lse.tolist()) if abs(lse) > 32]
+    near = [v for v in range(len(values)) if v not in far]
+    assert len(far) >= 8 and len(near) >= 4
+    rel = (4 * math.log2(vocab) + 4 + 2) * u
+    for rows, off in ((far, rel), (near, rel + 2.0 ** -20)):
+        assert float((d[rows, :-1] + p).abs().max()) <= off * p
+        assert float((d[rows, -1] - (1 - p)).abs().max()) <= off * p + 2 * u
+
+
 def test_gradient_against_differences():
     import tcu_scope_b200 as tcu
     x, t = make(3, 11, F32, 8, spread=1.0)
