@@ -92,6 +92,117 @@ def test_packed_sequences_match_reference(gate, wide, dim):
     assert tcu.device_error() == 0
 
 
+TYPES = [(F32, F32), (BF16, BF16), (F32, BF16), (F16, F16), (F32, F16)]
+
+
+def device_inputs(gate, shape, a_type, x_type, seed):
+    """As inputs(), made on the GPU: many columns."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    if gate == "sigmoid":
+        a = 3 + 2 * n(*shape)
+    else:
+        a = -torch.exp(-3 + 1.5 * n(*shape))
+        a = a.exp() * torch.sign(n(*shape) + 1.5) if gate == "decay" else a
+    return a.to(a_type), n(*shape).to(x_type), n
+
+
+def some_channels(dim):
+    """The ends of the columns of 64, and others."""
+    return sorted({c for c in (0, 1, 63, 64, 127, dim // 2, dim // 3, dim - 65, dim - 2, dim - 1) if 0 <= c < dim})
+
+
+def check_channels(gate, a, x, h0, dh, dlast, got, what):
+    """check_batch() at some channels, those of all sequences side by side."""
+    batch, tokens, dim = x.shape
+    ch = some_channels(dim)
+    pick = lambda t: t[..., ch].double().cpu()  # noqa: E731
+    rows = lambda t: pick(t).transpose(0, 1).reshape(tokens, -1)  # noqa: E731
+    flat = lambda t: pick(t).reshape(-1)  # noqa: E731
+    want = ref.linear_scan(gate, rows(a), rows(x), flat(h0), rows(dh), flat(dlast))
+    for name, t in got.items():
+        t = t[..., ch].reshape(-1) if name in ("last", "dh0") else t[..., ch].transpose(0, 1).reshape(tokens, -1)
+        ref.assert_within(t, *want[name], (what, name))
+
+
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("a_type,x_type", TYPES)
+@pytest.mark.parametrize("batch,dim", [(37, 2048), (36, 2057)])
+def test_a_warp_for_each_of_many_columns(gate, a_type, x_type, batch, dim):
+    """Where there are eight columns for every SM the gradient goes through a sequence with one warp: windows of 32
+    rows with two states each, a ring that wraps, lengths around the borders of both."""
+    import tcu_scope_b200 as tcu
+    for tokens in (33, 47, 64, 65, 289) if a_type == x_type else (31, 177):
+        a, x, n = device_inputs(gate, (batch, tokens, dim), a_type, x_type, tokens)
+        h0, dlast, dh = n(batch, dim), n(batch, dim), n(batch, tokens, dim).to(x_type)
+        got = run_batch(tcu, gate, a, x, h0, dh, dlast)
+        check_channels(gate, a, x, h0, dh, dlast, got, (gate, tokens))
+        again = run_batch(tcu, gate, a, x, h0, dh, dlast)
+        assert all(torch.equal(got[k], again[k]) for k in got)
+
+
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("a_type,x_type", TYPES)
+@pytest.mark.parametrize("batch,tokens,dim", [(8, 300, 1280), (8, 1111, 1210), (3, 2050, 3200)])
+def test_a_block_for_each_column(gate, a_type, x_type, batch, tokens, dim):
+    """As many columns as SMs and more: the warps of one block share a sequence, with several windows each."""
+    import tcu_scope_b200 as tcu
+    a, x, n = device_inputs(gate, (batch, tokens, dim), a_type, x_type, tokens)
+    h0, dlast, dh = n(batch, dim), n(batch, dim), n(batch, tokens, dim).to(x_type)
+    got = run_batch(tcu, gate, a, x, h0, dh, dlast)
+    check_channels(gate, a, x, h0, dh, dlast, got, (gate, tokens))
+
+
+def lengths_of(kind):
+    """Lengths of packed sequences: at and above the number that is ranked, and batches whose mean says little."""
+    g = torch.Generator().manual_seed(len(kind))
+    if kind in ("96", "97", "300"):
+        n = int(kind)
+        lengths = torch.randint(0, 60, (n,), generator=g)
+        lengths[torch.rand(n, generator=g) < 0.1] = 0
+        lengths[n // 3], lengths[n - 1], lengths[5] = 700, 150, 0
+        return lengths.tolist()
+    if kind == "1100":
+        return torch.randint(0, 5, (1100,), generator=g).tolist()
+    return [5] * 20 + [0, 350, 1] + [3] * 27 if kind == "one long" else [2000] + [32] * 30
+
+
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("a_type,x_type", [(BF16, BF16), (F32, F16), (F32, F32)])
+@pytest.mark.parametrize("kind", ["96", "97", "300", "1100", "one long", "long first"])
+@pytest.mark.parametrize("dim", [72, 1033, 2048])
+def test_packed_batches_match_reference(gate, a_type, x_type, kind, dim):
+    import tcu_scope_b200 as tcu
+    lengths = lengths_of(kind)
+    first, rest = 3, 9
+    ends = torch.tensor([first] + lengths).cumsum(0)
+    tokens, batch = int(ends[-1]) + rest, len(lengths)
+    a, x, n = device_inputs(gate, (tokens, dim), a_type, x_type, dim)
+    h0, dlast, dh = n(batch, dim), n(batch, dim), n(tokens, dim).to(x_type)
+    offsets = ends.to(torch.int32).cuda()
+
+    def run():
+        states = tcu.linear_scan_states(x, offsets)
+        h, last = tcu.linear_scan(a, x, gate=gate, h0=h0, offsets=offsets, states=states)
+        da, dx, dh0 = tcu.linear_scan_backward(dh, a, x, states, gate=gate, dlast=dlast, offsets=offsets)
+        return dict(h=h, last=last, da=da, dx=dx, dh0=dh0)
+
+    got = run()
+    ch = some_channels(dim)
+    cpu = {k: t[..., ch].double().cpu() for k, t in dict(a=a, x=x, h0=h0, dh=dh, dlast=dlast).items()}
+    few = {k: t[..., ch] for k, t in got.items()}
+    for k in ("h", "da", "dx"):
+        assert bool((got[k][:first] == 0).all()) and bool((got[k][tokens - rest:] == 0).all())
+    long = [b for b in range(batch) if lengths[b] > 100]
+    for b in sorted({*long, *range(0, batch, 1 + batch // 40), 5, batch - 1}):
+        i, j = int(ends[b]), int(ends[b + 1])
+        want = ref.linear_scan(gate, cpu["a"][i:j], cpu["x"][i:j], cpu["h0"][b], cpu["dh"][i:j], cpu["dlast"][b])
+        check(dict(h=few["h"][i:j], da=few["da"][i:j], dx=few["dx"][i:j], last=few["last"][b], dh0=few["dh0"][b]), want, (gate, b))
+    again = run()
+    assert all(torch.equal(got[k], again[k]) for k in got)
+    assert tcu.device_error() == 0
+
+
 def test_strided_and_unaligned_inputs():
     """a and x as column blocks of one projection, a shifted view, a gate broadcast over the batch."""
     import tcu_scope_b200 as tcu
