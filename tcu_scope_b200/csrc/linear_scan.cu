@@ -56,9 +56,9 @@ linear_scan_step_kernel(const StepArgs p) {
 
 // ------------------------------------------------------------------ host side
 
-// Whether rows that begin at p, a row (and a batch) stride apart, can be read VEC elements at a time.
-bool vector_rows(const void* p, size_t elem, int64_t batch_stride, int64_t row_stride, int vec) {
-  return aligned(p, elem * vec) && batch_stride % vec == 0 && row_stride % vec == 0;
+// Whether rows that begin at p, a row stride apart, can be read VEC elements at a time.
+bool vector_rows(const void* p, size_t elem, int64_t row_stride, int vec) {
+  return aligned(p, elem * vec) && row_stride % vec == 0;
 }
 
 template <typename F>
@@ -173,7 +173,7 @@ int tcu_linear_scan_step(const tcu_linear_scan_step_args* g, void* stream) {
   p.batch = g->batch, p.pool = g->pool, p.dim = g->dim, p.a_row = g->a_row_stride, p.x_row = g->x_row_stride;
   p.wide = g->slots_are_64bit != 0, p.clear_rest = g->clear_rest != 0;
   auto fits = [&](int v) {
-    return p.dim % v == 0 && vector_rows(p.a, ea, 0, p.a_row, v) && vector_rows(p.x, e, 0, p.x_row, v) &&
+    return p.dim % v == 0 && vector_rows(p.a, ea, p.a_row, v) && vector_rows(p.x, e, p.x_row, v) &&
            aligned(p.h, e * v) && aligned(p.state, 4 * v);
   };
   const cudaError_t err = for_type(g->type, [&](auto t) {

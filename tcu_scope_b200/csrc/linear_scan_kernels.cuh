@@ -10,9 +10,10 @@
 // A warp copies its rows into a ring of its own in shared memory (cp.async, 16 bytes a lane) and waits for
 // nothing but its own copies and its neighbours' maps.  What that costs: one warp alone issues an instruction every 3.5
 // cycles, so 64 channels of 2048 tokens take one warp 90 us and 8 warps an SM are wanted; the backward pass
-// of 1184 columns of 64 channels and more is one warp per column, without maps (118 us against 156 for 64 x 512 x 2048).
-// Measured, bf16, of the copy bandwidth: 64 x 512 x 2048 89 % forward, 84 % backward; 8 x 2048 x 2560 (320 columns, so that
-// some SMs have three and some two) 72 % and 66 %; 1 x 65537 x 1024 (16 columns, clusters of 8, one meeting of the
+// of 1184 columns of 64 channels and more is one warp per column, without maps (113 us for 64 x 512 x 2048; 156 with
+// maps, when one warp took 118).
+// Measured, bf16, of the copy bandwidth: 64 x 512 x 2048 89 % forward, 90 % backward; 8 x 2048 x 2560 (320 columns, so that
+// some SMs have three and some two) 73 % and 67 %; 1 x 65537 x 1024 (16 columns, clusters of 8, one meeting of the
 // cluster for 1024 rows) 42 %.
 //
 // Backwards, with g_t = f_t dh_t passing from row t to row t-1 (dh_t = dy_t + g_{t+1}), the same
@@ -39,7 +40,7 @@ constexpr int kMaxWarps   = 8;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxStages  = 3;   // windows in a warp's ring
 // Blocks of 8 warps that the registers of an SM hold.  The gradient of SIGMOID gates spills 400 bytes a thread at 128
-// registers, and is faster with half the warps (packed fp16, 37 sequences of 1000 channels: 165 us against 233).
+// registers, and is faster with half the warps (packed fp16, 37 sequences of 1000 channels: 82 us against 112).
 constexpr int kForwardBlocks = 2;
 template <int GATE>
 constexpr int kBackwardBlocks = GATE == TCU_GATE_SIGMOID ? 1 : 2;
@@ -138,7 +139,7 @@ __device__ __forceinline__ bool search_finds(const ScanArgs& p, uint32_t b, int6
 // order among themselves, and of the others those run that are in order with all.  By all threads of a block, when its
 // first rows are on their way, and through shared memory: values that the compiler does not know to be one for the
 // block make the gradient's loop spill.  (bf16, forward + backward, and without the search: 4000 sequences of 10 x 1024 359 + 272
-// us, 312 + 249; 300 of 67 x 2048 75 + 107, 72 + 110; 97 of 206 x 2048 62 + 129, 59 + 136.)
+// us, 312 + 249; 300 of 67 x 2048 75 + 106, 72 + 110; 97 of 206 x 2048 61 + 127, 59 + 136.)
 __device__ __forceinline__ void leave_out(const ScanArgs& p, int64_t b, int& left_out) {
   if (p.batch > kRankedBatch) {
     if (threadIdx.x < 32) {
@@ -288,7 +289,7 @@ struct Map {  // h -> a h + b, of a lane's two channels
   float2 a, b;
 };
 
-// What both kernels begin with: a block's place.
+// What the backward kernel begins with: a block's place.  (The forward kernel has its own variables for it.)
 struct Place {
   int64_t b, first, ch;  // sequence, the block's first channel, the lane's
   int left, count;       // channels of the block from `first`; of the lane: above 0, above 1

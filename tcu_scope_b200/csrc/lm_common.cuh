@@ -20,13 +20,10 @@ constexpr int kMaxDevices = 64;
 // range or named twice; what it names was left out.
 constexpr unsigned kErrIndex = 8u;
 
-// One word for each of the three translation units; tcu_device_error() joins them.
+// One word for each translation unit; tcu_device_error() joins those of the units that raise it (all but norm_residual.cu).
 static __device__ unsigned int g_lm_error_word;
 
 __device__ __forceinline__ void raise_index_error() { atomicOr(&g_lm_error_word, kErrIndex); }
-
-// Bit 0, as in the other kernels: an mbarrier wait ran out.
-constexpr unsigned kErrBarrier = 1u;
 
 // ------------------------------------------------------------------ elements
 // (16 bytes are the widest access: longer vectors are several of them)
@@ -120,15 +117,12 @@ __device__ __forceinline__ void copy_async4(void* to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Returns when all but the newest `pending` groups of this thread have arrived.
+// Returns when all but the newest `pending` groups of this thread, 2 at most, have arrived.
 __device__ __forceinline__ void copy_wait(int pending) {
   switch (pending) {
     case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
     case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
   }
 }
 

@@ -20,10 +20,12 @@
 //
 // Bound by HBM: 4 arrays forward, 6 backward.  Rows come through a ring in shared memory, each thread copying (cp.async)
 // what it will read itself: nothing is waited for but a thread's own copies and the one meeting.
-// Measured, of the copy bandwidth: forward 16384 x 4096 bf16 105 us (77 %), 65536 x 256 81 % (a warp a row, no meeting),
-// bound by the instructions a row takes; gradient 225 us (54 %), of which its seven sums take 62: it needs 127 registers, so
-// that one block of 512 threads is on an SM and nothing runs while that meets.  (Two meetings forward and four
-// backward took 129 and 509 us; pairs of floats in one instruction 131 and 237.)
+// Measured, bf16, of the copy bandwidth: forward 16384 x 4096 106 us (77 %; without post and gate 103, without residual, too,
+// 88), 65536 x 256 80 % (a warp a row, no meeting), 8192 x 5120 65 %, bound by the instructions a row takes; gradient 226 us (54 %;
+// 218, 190), of which its seven sums take 62: it needs up to 127 registers, so that one block of 512 threads is on an SM and
+// nothing runs while that meets.  Gradient of rows a warp holds, 65536 x 256, 39 %; of 16 elements a thread, 8192 x 5120, 34 %;
+// element by element, 4096 x 12288, 15 %.  (Two meetings forward and four backward took 129 and 509 us; pairs of
+// floats in one instruction 131 and 237.)
 #include <type_traits>
 
 #include "lm_common.cuh"
@@ -128,8 +130,9 @@ __device__ __forceinline__ void store_part(T* row, const Part<VEC, E>& t, const 
 
 constexpr int kStages = 3;  // rows in the ring
 
-// An array's rows on their way through the ring (VEC == 1: read from where they are; those rows are not
-// aligned for copies).
+// An array's rows on their way through the ring (VEC == 1: read from where they are, an element at a time; those rows are not
+// aligned for copies, or the ring does not hold them, which 16-byte loads past the ring would not need: not built).
+// The gate's rows do not take it: with a gate for each row each row waits for its gate, too.
 template <typename T, int VEC, int E>
 struct Stream {
   const T* base;
@@ -434,8 +437,10 @@ int row_threads(int64_t dim, int e) { return int((dim + e * 32 - 1) / (e * 32) *
 // Elements per thread: 8, but not more threads than `most`.
 int elements(int64_t dim, int most) { return dim <= most * 8 ? 8 : 16; }
 
-// Workers of the backward pass, which needs 100 registers and more: as many as 512 threads on each of the 148 SMs
-// are (a number that leaves some SMs with one more than others takes twice as long: 236 blocks of 320 threads).
+// Workers of the backward pass, which needs 122 registers and more: as many as 512 threads on each of the 148 SMs
+// are (a number that leaves some SMs with one more than others takes twice as long: 236 blocks of 320 threads).  Rows of up to 256
+// elements are 296 blocks of 8 warps, of which the 146 ... 164 registers a thread that their kernels take let an SM
+// hold one at a time; above 4096 elements the kernels spill (480 bytes a thread, 1200 above 8192).
 int64_t backward_workers(int64_t dim) {
   const int threads = dim <= kWarpDim ? 32 : row_threads(dim, elements(dim, 512));
   return threads > 512 ? 148 : 148 * (512 / threads);
@@ -465,7 +470,7 @@ int launch_rows(K kernel, bool* configured, NormArgs p, int elem, int vec, int a
   return cudaGetLastError() == cudaSuccess ? TCU_OK : TCU_ERR_CUDA;
 }
 
-// Whether a ring of rows of `arrays` arrays fits into shared memory.
+// Whether a ring of rows of `arrays` arrays fits into shared memory (two of 32 bits: up to 9212 elements, four: 4604).
 bool ring_fits(int64_t dim, size_t elem, int arrays) { return kStages * arrays * (dim * int64_t(elem) + 15) / 16 * 16 <= kMostShared; }
 
 bool row_vectors(const void* p, size_t elem, int64_t stride, int vec) {
@@ -642,7 +647,8 @@ int tcu_norm_residual_backward(const tcu_norm_residual_backward_args* g, void* s
         static bool ready[kMaxDevices];
         return launch_rows(norm_residual_backward_kernel<T, W, VEC, 16, false, 512>, ready, p, sizeof(T), VEC, 4, 1, grid, threads, st);
       }
-      // (a ring of rows of more than 8192 elements does not fit with four arrays of 32 bits)
+      // (a ring of rows of more than 8192 elements does not fit with four arrays of 32 bits, of 16 bits up to 9209: read
+      // element by element, whatever their type and alignment)
       static bool ready[kMaxDevices];
       return launch_rows(norm_residual_backward_kernel<T, W, 1, 16, false, 1024>, ready, p, sizeof(T), 1, 4, 1, grid, threads, st);
     };
