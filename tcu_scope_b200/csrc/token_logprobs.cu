@@ -14,8 +14,8 @@
 //
 // A row is read by the P blocks of a cluster, P > 1 where there are few rows, which join their sums
 // and lists in shared memory of the first.  Bound by HBM: one read forward, a read and a write backward.
-// Measured, bf16: 4096 x 128000 174 us (92 % of the copy bandwidth) without, 211 us with 8 alternatives: 83 % of the issue slots
-// are taken, by 9 instructions an element and the exponentials' unit at 16 a cycle; gradient of 2048 x 100003 141 us (88 %).
+// Measured, bf16: 4096 x 128000 164 ... 175 us (97 ... 91 % of the copy bandwidth) without, 212 us with 8 alternatives: 64 % of
+// the issue slots are taken, and 56 % of what the exponentials' unit can do; gradient of 2048 x 100003 141 us (88 %).
 #include <cooperative_groups.h>
 
 #include <type_traits>
